@@ -46,7 +46,8 @@ enum {
     RTD_ERR_PEER_TIMEOUT = 7,  /* a bounded cross-GPU wait gave up */
     RTD_ERR_INDEX = 8,         /* an embedding id was out of range */
     RTD_ERR_DEVICE = 9,        /* a kernel raised the context's device status word */
-    RTD_ERR_WORKSPACE = 10     /* the call needs more scratch than the context reserved */
+    RTD_ERR_WORKSPACE = 10,    /* the call needs more scratch than the context reserved */
+    RTD_ERR_CACHE = 11         /* paged cache: a block, slot or length out of range, or no free blocks */
 };
 
 /* GGML type ids (crates/runtimed-gguf/src/quant/dtype.rs:27-46), and the id this library
@@ -222,6 +223,78 @@ rtd_status rtd_qlinear_argmax(rtd_ctx* ctx, const rtd_qweight* w, const void* x,
 rtd_status rtd_qlinear_argmax_keys(rtd_ctx* ctx, const rtd_qweight* w, const void* x, uint32_t x_dtype,
                                    int64_t ldx, int64_t M, const float* bias, int64_t row0, uint64_t* keys,
                                    void* stream);
+
+/* ---- the paged KV cache in 4 bits --------------------------------------------
+ * No counterpart in the reference (its caches hold 16 or 32 bits).  A decode step that
+ * never waits for the host: rtd_kv_plan, then per layer rtd_rope_kv4_append and
+ * rtd_attention_kv4, then the LM head and rtd_sample, all captured in one CUDA graph.
+ *
+ * pages is uint8 [num_blocks][n_kv][20 * head_dim], 16-byte aligned: a page holds 16
+ * tokens of one kv head, every 32 dims of a token as 32 codes of 4 bits with a step d and
+ * a minimum m in f16, x ~ d * code + m, d = f16((max - min) / 15), m = f16(min), code =
+ * (x - m) / d rounded to even and kept within 0..15.  A group that holds an infinity or
+ * NaN, or whose d or m overflows f16, reads as NaN.  head_dim is 32, 64, 96 or 128;
+ * any whole number of query heads per kv head.
+ * A slot is block * 16 + offset: token p of sequence s lies in slot
+ * block_table[s][p / 16] * 16 + p % 16.  What a kernel finds out of range (a block or
+ * slot outside the pool, a length beyond its bound) raises RTD_ERR_CACHE in the device
+ * status word; nothing outside the buffers is touched. */
+rtd_status rtd_kv4_page_bytes(int32_t head_dim, int64_t* bytes);
+
+/* Brings S sequences (at most 8192) from length[s] to want[s] tokens, on the device.
+ * Sequences that shrink give their blocks back to the free stack (last block first, in
+ * sequence order), then those that grow take blocks from its top: the order of the host's
+ * PagedKvCache.  length, block_table [S][max_blocks], free_list [num_blocks] (the first
+ * *free_count entries are free) and free_count are updated in place; table entries past a
+ * sequence's length are left as they were.
+ * The tokens of the growing sequences are listed by sequence and position: q_start [S + 1]
+ * (first token of each sequence), tok_seq / tok_pos / tok_slot [max_tokens] with -1 behind
+ * the last token (rtd_rope_kv4_append writes no key or value for such a row).  The four
+ * may be NULL together.  After the call length is rtd_attention_kv4's ctx_len.
+ * A want below 0 or above 16 * max_blocks, more tokens than max_tokens or too few free
+ * blocks raise RTD_ERR_CACHE: the state then stays as it was and the lists are empty. */
+rtd_status rtd_kv_plan(rtd_ctx* ctx, const int32_t* want, int32_t S, int32_t* length, int32_t* block_table,
+                       int32_t max_blocks, int32_t* free_list, int32_t* free_count, int32_t num_blocks,
+                       int32_t* q_start, int32_t* tok_seq, int32_t* tok_pos, int32_t* tok_slot, int32_t max_tokens,
+                       void* stream);
+
+/* rtd_rope_kv_append into 4-bit pages: NeoX rope over the first rot_dim dims of queries and
+ * keys by the angles tok_pos[t] * inv_freq[i] (f64 [rot_dim / 2] on the device, e.g.
+ * theta^(-2i / rot_dim); formed in 64 bits), queries to q_out f32 [T][n_head][head_dim],
+ * keys and values quantised into slot tok_slot[t].  Rows with a negative slot only rotate
+ * their queries.  Two tokens of a call must not share a slot. */
+rtd_status rtd_rope_kv4_append(rtd_ctx* ctx, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                               int64_t ldv, uint32_t x_dtype, int64_t T, int32_t n_head, int32_t n_kv,
+                               int32_t head_dim, int32_t rot_dim, const double* inv_freq, const int32_t* tok_pos,
+                               const int32_t* tok_slot, void* pages, int32_t num_blocks, float* q_out, void* stream);
+
+/* k, v [n][n_kv][head_dim] = the values held in slots[0..n) (zeros for a negative slot). */
+rtd_status rtd_kv4_read(rtd_ctx* ctx, const int32_t* slots, int64_t n, int32_t n_kv, int32_t head_dim,
+                        const void* pages, int32_t num_blocks, void* k, void* v, uint32_t dtype, void* stream);
+
+/* Causal GQA over 4-bit pages.  Sequence s has the queries q_start[s] .. q_start[s + 1] - 1
+ * (rows of q, ldq apart) at its last positions: the i-th of n sees the keys
+ * 0 .. ctx_len[s] - n + i; a row that sees none is written as zeros, a row of no sequence
+ * is left alone.  max_q and max_ctx bound the queries and the length of any sequence.
+ * o rows are ldo apart.  Long contexts are split over CTAs and joined in order, so equal
+ * calls give equal bits. */
+rtd_status rtd_attention_kv4(rtd_ctx* ctx, const void* q, uint32_t q_dtype, int64_t ldq, int64_t T, int32_t n_head,
+                             int32_t n_kv, int32_t head_dim, float scale, const int32_t* q_start,
+                             const int32_t* ctx_len, int32_t S, const int32_t* block_table, int32_t max_blocks,
+                             int32_t max_q, int32_t max_ctx, const void* pages, int32_t num_blocks, void* o,
+                             uint32_t o_dtype, int64_t ldo, void* stream);
+
+/* ids[t] drawn from row t of logits [T, V] (V at most 2^19) with the random number u[t] in
+ * [0, 1): weights w_n = rint(2^44 exp((x_n - max) / temperature)); the top_k largest stay,
+ * of these the fewest whose weight reaches floor(top_p * sum), of these those with
+ * w_n >= min_p * 2^44 (equal logits: lowest index first); the pick is the lowest n whose
+ * running sum over what stayed exceeds floor(u * sum).  temperature, top_k, top_p and min_p
+ * are device arrays [T] or NULL (1, off, off, off); top_k <= 0, top_p >= 1 and min_p <= 0
+ * are off.  A NaN logit is never chosen.  The lowest index of the maximum is taken (as
+ * rtd_argmax does) when temperature is not above 0, top_k is 1 or the maximum is infinite. */
+rtd_status rtd_sample(rtd_ctx* ctx, const void* logits, uint32_t dtype, int64_t ldx, int64_t T, int64_t V,
+                      const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                      const float* u, int32_t* ids, void* stream);
 
 /* ---- tensor-parallel row reduction -----------------------------------------
  * Replaces RowParallelLinear::forward + ring_all_reduce

@@ -23,6 +23,7 @@ RTD_ERR_PEER_TIMEOUT = 7
 RTD_ERR_INDEX = 8
 RTD_ERR_DEVICE = 9
 RTD_ERR_WORKSPACE = 10
+RTD_ERR_CACHE = 11
 
 TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 8, 12, 14
 TYPE_INT4_MARLIN = 1001  # rtd_marlin_upload handles (not a GGUF type)
@@ -67,6 +68,16 @@ SIGNATURES = {
     "rtd_argmax": (_c.c_int32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp]),
     "rtd_qlinear_argmax": (_c.c_int32, [_vp, _vp, _vp, _u32, _i64, _i64, _vp, _vp, _u32, _i64, _vp, _vp]),
     "rtd_qlinear_argmax_keys": (_c.c_int32, [_vp, _vp, _vp, _u32, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "rtd_kv4_page_bytes": (_c.c_int32, [_c.c_int32, _c.POINTER(_i64)]),
+    "rtd_kv_plan": (_c.c_int32, [_vp, _vp, _c.c_int32, _vp, _vp, _c.c_int32, _vp, _vp, _c.c_int32, _vp, _vp, _vp, _vp,
+                                 _c.c_int32, _vp]),
+    "rtd_rope_kv4_append": (_c.c_int32, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _u32, _i64, _c.c_int32, _c.c_int32,
+                                         _c.c_int32, _c.c_int32, _vp, _vp, _vp, _vp, _c.c_int32, _vp, _vp]),
+    "rtd_kv4_read": (_c.c_int32, [_vp, _vp, _i64, _c.c_int32, _c.c_int32, _vp, _c.c_int32, _vp, _vp, _u32, _vp]),
+    "rtd_attention_kv4": (_c.c_int32, [_vp, _vp, _u32, _i64, _i64, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_float,
+                                       _vp, _vp, _c.c_int32, _vp, _c.c_int32, _c.c_int32, _c.c_int32, _vp,
+                                       _c.c_int32, _vp, _u32, _i64, _vp]),
+    "rtd_sample": (_c.c_int32, [_vp, _vp, _u32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "rtd_qembed": (_c.c_int32, [_vp, _vp, _vp, _i64, _vp, _vp]),
     "rtd_qdequant": (_c.c_int32, [_vp, _vp, _vp, _vp]),
     "rtd_fp8weight_upload": (_c.c_int32, [_vp, _vp, _vp, _i64, _i64, _i64, _c.POINTER(_vp)]),

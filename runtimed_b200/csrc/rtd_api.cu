@@ -28,6 +28,8 @@ struct rtd_ctx {
   int* status = nullptr;
   // rtd_qlinear_argmax's epilogue state: [4] packed keys and a CTA count, zero between calls
   unsigned long long* amax = nullptr;
+  // rtd_attention_kv4's CTAs-done words, zero between calls
+  unsigned* attn_count = nullptr;
   std::string err;
 };
 
@@ -62,6 +64,7 @@ constexpr size_t kWorkspaceBytes = 64ull << 20;  // activation staging (GEMV pre
 // the four-column GEMV pass is slower than one TN = 16 GEMM tile from M = 4 on, and
 // faster up to M = 3
 constexpr int64_t kGemmMinTokens = 4;
+constexpr size_t kAttnCountBytes = 64 << 10;
 constexpr size_t kAmaxBytes = 64;  // rtd_ctx::amax: 4 keys of 8 bytes, the count, padding
 
 thread_local std::string g_thread_err;
@@ -157,10 +160,13 @@ rtd_status rtd_init(int device, rtd_ctx** out) {
   if ((e = cudaMalloc(&c->ws, kWorkspaceBytes)) != cudaSuccess ||
       (e = cudaMalloc(&c->status, sizeof(int))) != cudaSuccess ||
       (e = cudaMemset(c->status, 0, sizeof(int))) != cudaSuccess ||
-      (e = cudaMalloc(&c->amax, kAmaxBytes)) != cudaSuccess || (e = cudaMemset(c->amax, 0, kAmaxBytes)) != cudaSuccess) {
+      (e = cudaMalloc(&c->amax, kAmaxBytes)) != cudaSuccess || (e = cudaMemset(c->amax, 0, kAmaxBytes)) != cudaSuccess ||
+      (e = cudaMalloc(&c->attn_count, kAttnCountBytes)) != cudaSuccess ||
+      (e = cudaMemset(c->attn_count, 0, kAttnCountBytes)) != cudaSuccess) {
     cudaFree(c->ws);
     cudaFree(c->status);
     cudaFree(c->amax);
+    cudaFree(c->attn_count);
     delete c;
     return fail(nullptr, RTD_ERR_OOM, "rtd_init: workspace allocation failed: %s", cudaGetErrorString(e));
   }
@@ -175,6 +181,7 @@ rtd_status rtd_destroy(rtd_ctx* ctx) {
   cudaFree(ctx->ws);
   cudaFree(ctx->status);
   cudaFree(ctx->amax);
+  cudaFree(ctx->attn_count);
   delete ctx;
   return RTD_OK;
 }
@@ -192,6 +199,8 @@ rtd_status rtd_check_device_status(rtd_ctx* ctx, void* stream) {
     if (v == RTD_ERR_INDEX) return fail(ctx, RTD_ERR_INDEX, "embedding id out of range");
     if (v == RTD_ERR_PEER_TIMEOUT)
       return fail(ctx, RTD_ERR_PEER_TIMEOUT, "a tensor-parallel peer did not arrive within the wait budget");
+    if (v == RTD_ERR_CACHE)
+      return fail(ctx, RTD_ERR_CACHE, "paged cache: a block, slot or length out of range, or no free blocks");
     return fail(ctx, RTD_ERR_DEVICE, "device status word raised code %d", v);
   }
   return RTD_OK;
@@ -702,6 +711,152 @@ rtd_status rtd_argmax(rtd_ctx* ctx, const float* x, int64_t ldx, int64_t T, int6
   if (ldx < V) return fail(ctx, RTD_ERR_SHAPE, "%s: ldx below V", who);
   DeviceGuard g(ctx->device);
   cudaError_t e = rtd::launch_argmax(x, ldx, T, V, out, (cudaStream_t)stream);
+  return e == cudaSuccess ? RTD_OK : cuda_fail(ctx, e, who);
+}
+
+// ---- the paged KV cache in 4 bits, and sampling ------------------------------
+namespace {
+rtd_status check_heads4(rtd_ctx* ctx, int32_t n_head, int32_t n_kv, int32_t head_dim, const char* who) {
+  if (n_head <= 0 || n_kv <= 0 || n_head % n_kv != 0)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: %d query heads are not a multiple of %d kv heads", who, n_head, n_kv);
+  if (head_dim <= 0 || head_dim % 32 != 0 || head_dim > 128)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: head_dim %d (32, 64, 96 or 128)", who, head_dim);
+  return RTD_OK;
+}
+rtd_status check_pool(rtd_ctx* ctx, const void* pages, int32_t num_blocks, const char* who) {
+  if (!pages) return fail(ctx, RTD_ERR_INVALID, "%s: NULL pointer", who);
+  if (reinterpret_cast<uintptr_t>(pages) % 16) return fail(ctx, RTD_ERR_INVALID, "%s: pages are not 16-byte aligned", who);
+  if (num_blocks <= 0 || num_blocks > INT32_MAX / 16)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: %d blocks (1 to %d)", who, num_blocks, INT32_MAX / 16);
+  return RTD_OK;
+}
+}  // namespace
+
+rtd_status rtd_kv4_page_bytes(int32_t head_dim, int64_t* bytes) {
+  if (!bytes) return fail(nullptr, RTD_ERR_INVALID, "rtd_kv4_page_bytes: NULL pointer");
+  if (head_dim <= 0 || head_dim % 32 != 0 || head_dim > 128)
+    return fail(nullptr, RTD_ERR_SHAPE, "rtd_kv4_page_bytes: head_dim %d (32, 64, 96 or 128)", head_dim);
+  *bytes = 20 * (int64_t)head_dim;
+  return RTD_OK;
+}
+
+rtd_status rtd_kv_plan(rtd_ctx* ctx, const int32_t* want, int32_t S, int32_t* length, int32_t* block_table,
+                       int32_t max_blocks, int32_t* free_list, int32_t* free_count, int32_t num_blocks,
+                       int32_t* q_start, int32_t* tok_seq, int32_t* tok_pos, int32_t* tok_slot, int32_t max_tokens,
+                       void* stream) {
+  const char* who = "rtd_kv_plan";
+  if (!ctx) return fail(nullptr, RTD_ERR_INVALID, "%s: ctx is NULL", who);
+  if (S < 0 || S > rtd::kPlanMaxSeqs)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: %d sequences (at most %d)", who, S, rtd::kPlanMaxSeqs);
+  if (max_tokens < 0) return fail(ctx, RTD_ERR_SHAPE, "%s: max_tokens is negative", who);
+  if (max_blocks <= 0 || max_blocks > INT32_MAX / 32 || num_blocks <= 0 || num_blocks > INT32_MAX / 16)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: a table of %d blocks a sequence, %d in all", who, max_blocks, num_blocks);
+  const bool lists = q_start || tok_seq || tok_pos || tok_slot;
+  if (lists && (!q_start || (max_tokens > 0 && (!tok_seq || !tok_pos || !tok_slot))))
+    return fail(ctx, RTD_ERR_INVALID, "%s: the token lists are given together or not at all", who);
+  if (!free_count || !free_list || (S > 0 && (!want || !length || !block_table)))
+    return fail(ctx, RTD_ERR_INVALID, "%s: NULL pointer", who);
+  DeviceGuard g(ctx->device);
+  if (g.err != cudaSuccess) return cuda_fail(ctx, g.err, who);
+  cudaError_t e = rtd::launch_kv_plan(want, S, length, block_table, max_blocks, free_list, free_count, num_blocks,
+                                      q_start, tok_seq, tok_pos, tok_slot, max_tokens, ctx->status,
+                                      (cudaStream_t)stream);
+  return e == cudaSuccess ? RTD_OK : cuda_fail(ctx, e, who);
+}
+
+rtd_status rtd_rope_kv4_append(rtd_ctx* ctx, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                               int64_t ldv, uint32_t x_dtype, int64_t T, int32_t n_head, int32_t n_kv,
+                               int32_t head_dim, int32_t rot_dim, const double* inv_freq, const int32_t* tok_pos,
+                               const int32_t* tok_slot, void* pages, int32_t num_blocks, float* q_out, void* stream) {
+  const char* who = "rtd_rope_kv4_append";
+  if (!ctx) return fail(nullptr, RTD_ERR_INVALID, "%s: ctx is NULL", who);
+  rtd_status st = check_heads4(ctx, n_head, n_kv, head_dim, who);
+  if (st != RTD_OK) return st;
+  if (rot_dim < 0 || rot_dim > head_dim || rot_dim % 2 != 0)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: rot_dim %d for head_dim %d", who, rot_dim, head_dim);
+  if (T < 0 || T > INT32_MAX) return fail(ctx, RTD_ERR_SHAPE, "%s: T=%lld", who, (long long)T);
+  if (T == 0) return RTD_OK;
+  if (!q || !k || !v || !tok_pos || !tok_slot || !q_out || (rot_dim > 0 && !inv_freq))
+    return fail(ctx, RTD_ERR_INVALID, "%s: NULL pointer", who);
+  if ((st = check_pool(ctx, pages, num_blocks, who)) != RTD_OK) return st;
+  if (!valid_dtype(x_dtype)) return fail(ctx, RTD_ERR_INVALID, "%s: bad dtype", who);
+  if (ldq < (int64_t)n_head * head_dim || ldk < (int64_t)n_kv * head_dim || ldv < (int64_t)n_kv * head_dim)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: row strides below the head widths", who);
+  DeviceGuard g(ctx->device);
+  if (g.err != cudaSuccess) return cuda_fail(ctx, g.err, who);
+  cudaError_t e = rtd::launch_rope_kv4(q, ldq, k, ldk, v, ldv, (int)x_dtype, T, n_head, n_kv, head_dim, rot_dim,
+                                       inv_freq, tok_pos, tok_slot, static_cast<uint8_t*>(pages), num_blocks, q_out,
+                                       ctx->sm_count, ctx->status, (cudaStream_t)stream);
+  return e == cudaSuccess ? RTD_OK : cuda_fail(ctx, e, who);
+}
+
+rtd_status rtd_kv4_read(rtd_ctx* ctx, const int32_t* slots, int64_t n, int32_t n_kv, int32_t head_dim,
+                        const void* pages, int32_t num_blocks, void* k, void* v, uint32_t dtype, void* stream) {
+  const char* who = "rtd_kv4_read";
+  if (!ctx) return fail(nullptr, RTD_ERR_INVALID, "%s: ctx is NULL", who);
+  rtd_status st = check_heads4(ctx, n_kv, n_kv, head_dim, who);
+  if (st != RTD_OK) return st;
+  if (n < 0) return fail(ctx, RTD_ERR_SHAPE, "%s: n is negative", who);
+  if (n == 0) return RTD_OK;
+  if (!slots || !k || !v) return fail(ctx, RTD_ERR_INVALID, "%s: NULL pointer", who);
+  if ((st = check_pool(ctx, pages, num_blocks, who)) != RTD_OK) return st;
+  if (!valid_dtype(dtype)) return fail(ctx, RTD_ERR_INVALID, "%s: bad dtype", who);
+  DeviceGuard g(ctx->device);
+  if (g.err != cudaSuccess) return cuda_fail(ctx, g.err, who);
+  cudaError_t e = rtd::launch_kv4_read(slots, n, n_kv, head_dim, static_cast<const uint8_t*>(pages), num_blocks, k, v,
+                                       (int)dtype, ctx->status, (cudaStream_t)stream);
+  return e == cudaSuccess ? RTD_OK : cuda_fail(ctx, e, who);
+}
+
+rtd_status rtd_attention_kv4(rtd_ctx* ctx, const void* q, uint32_t q_dtype, int64_t ldq, int64_t T, int32_t n_head,
+                             int32_t n_kv, int32_t head_dim, float scale, const int32_t* q_start,
+                             const int32_t* ctx_len, int32_t S, const int32_t* block_table, int32_t max_blocks,
+                             int32_t max_q, int32_t max_ctx, const void* pages, int32_t num_blocks, void* o,
+                             uint32_t o_dtype, int64_t ldo, void* stream) {
+  const char* who = "rtd_attention_kv4";
+  if (!ctx) return fail(nullptr, RTD_ERR_INVALID, "%s: ctx is NULL", who);
+  rtd_status st = check_heads4(ctx, n_head, n_kv, head_dim, who);
+  if (st != RTD_OK) return st;
+  if (T < 0 || T > INT32_MAX || S < 0) return fail(ctx, RTD_ERR_SHAPE, "%s: T=%lld S=%d", who, (long long)T, S);
+  if (T == 0 || S == 0) return RTD_OK;
+  if (!q || !q_start || !ctx_len || !block_table || !o || max_blocks <= 0)
+    return fail(ctx, RTD_ERR_INVALID, "%s: NULL pointer or no block table", who);
+  if ((st = check_pool(ctx, pages, num_blocks, who)) != RTD_OK) return st;
+  if (!valid_dtype(q_dtype) || !valid_dtype(o_dtype)) return fail(ctx, RTD_ERR_INVALID, "%s: bad dtype", who);
+  if (ldq < (int64_t)n_head * head_dim || ldo < (int64_t)n_head * head_dim)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: row strides below n_head * head_dim", who);
+  if (max_ctx <= 0 || (max_ctx + 15ll) / 16 > max_blocks)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: max_ctx %d outside the block table (%d blocks)", who, max_ctx, max_blocks);
+  if (max_q <= 0) return fail(ctx, RTD_ERR_SHAPE, "%s: max_q %d", who, max_q);
+  rtd::Kv4Attention c{q, (int)q_dtype, ldq, T, n_head, n_kv, head_dim, scale, q_start, ctx_len, S, block_table,
+                      max_blocks, max_q, max_ctx, static_cast<const uint8_t*>(pages), num_blocks, o, (int)o_dtype, ldo,
+                      ctx->ws, ctx->ws_bytes, ctx->attn_count, (int64_t)(kAttnCountBytes / sizeof(unsigned)),
+                      ctx->status, ctx->sm_count, (cudaStream_t)stream};
+  DeviceGuard g(ctx->device);
+  if (g.err != cudaSuccess) return cuda_fail(ctx, g.err, who);
+  int plan_err = 0;
+  cudaError_t e = rtd::launch_kv4_attention(c, &plan_err);
+  if (plan_err)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: %d sequences x %d kv heads x %d queries are more than a grid holds", who, S, n_kv, max_q);
+  return e == cudaSuccess ? RTD_OK : cuda_fail(ctx, e, who);
+}
+
+rtd_status rtd_sample(rtd_ctx* ctx, const void* logits, uint32_t dtype, int64_t ldx, int64_t T, int64_t V,
+                      const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                      const float* u, int32_t* ids, void* stream) {
+  const char* who = "rtd_sample";
+  if (!ctx) return fail(nullptr, RTD_ERR_INVALID, "%s: ctx is NULL", who);
+  if (T < 0 || T > INT32_MAX / 8 || V <= 0 || V > rtd::kSampleMaxVocab)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: T=%lld V=%lld (at most %lld)", who, (long long)T, (long long)V,
+                (long long)rtd::kSampleMaxVocab);
+  if (T == 0) return RTD_OK;
+  if (!logits || !u || !ids) return fail(ctx, RTD_ERR_INVALID, "%s: NULL pointer", who);
+  if (!valid_dtype(dtype)) return fail(ctx, RTD_ERR_INVALID, "%s: bad dtype", who);
+  if (ldx < V) return fail(ctx, RTD_ERR_SHAPE, "%s: ldx below V", who);
+  DeviceGuard g(ctx->device);
+  if (g.err != cudaSuccess) return cuda_fail(ctx, g.err, who);
+  cudaError_t e = rtd::launch_sample(logits, (int)dtype, ldx, T, V, temperature, top_k, top_p, min_p, u, ids,
+                                     (cudaStream_t)stream);
   return e == cudaSuccess ? RTD_OK : cuda_fail(ctx, e, who);
 }
 

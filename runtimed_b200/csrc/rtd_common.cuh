@@ -15,7 +15,7 @@
 namespace rtd {
 
 // Device status word codes (mirrors RTD_ERR_* of include/rtd.h).
-enum : int { kDevOk = 0, kDevPeerTimeout = 7, kDevIndex = 8, kDevWaitTimeout = 9 };
+enum : int { kDevOk = 0, kDevPeerTimeout = 7, kDevIndex = 8, kDevWaitTimeout = 9, kDevCache = 11 };
 
 __device__ __forceinline__ void raise_status(int* status, int code) {
   if (status) atomicCAS(status, 0, code);

@@ -161,6 +161,50 @@ cudaError_t launch_silu_mul(const void* gate, int gdt, int64_t ldg, const void* 
                             int64_t F, void* y, int ydt, int64_t ldy, cudaStream_t st);
 cudaError_t launch_argmax(const float* x, int64_t ldx, int64_t T, int64_t V, int* out, cudaStream_t st);
 
+// The 4-bit paged KV cache (rtd_kv4.cu).
+constexpr int kPlanMaxSeqs = 8192;  // their offsets fit one CTA's shared memory
+cudaError_t launch_kv_plan(const int* want, int S, int* length, int* table, int max_blocks, int* free_list,
+                           int* free_count, int num_blocks, int* q_start, int* tok_seq, int* tok_pos, int* tok_slot,
+                           int max_tokens, int* status, cudaStream_t st);
+cudaError_t launch_rope_kv4(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                            int x_dtype, int64_t T, int n_head, int n_kv, int head_dim, int rot_dim,
+                            const double* inv_freq, const int* tok_pos, const int* tok_slot, uint8_t* pages,
+                            int num_blocks, float* q_out, int sm_count, int* status, cudaStream_t st);
+cudaError_t launch_kv4_read(const int* slots, int64_t n, int n_kv, int head_dim, const uint8_t* pages, int num_blocks,
+                            void* k, void* v, int dtype, int* status, cudaStream_t st);
+struct Kv4Attention {
+  const void* q;
+  int q_dtype;
+  int64_t ldq, T;
+  int n_head, n_kv, head_dim;
+  float scale;
+  const int* q_start;
+  const int* ctx_len;
+  int S;
+  const int* block_table;
+  int max_blocks, max_q, max_ctx;
+  const uint8_t* pages;
+  int num_blocks;
+  void* o;
+  int o_dtype;
+  int64_t ldo;
+  float* ws;          // the chunks' partial states
+  size_t ws_bytes;
+  unsigned* count;    // CTAs done per tile, zero between calls (the last one clears its word)
+  int64_t count_words;
+  int* status;
+  int sm_count;
+  cudaStream_t stream;
+};
+// *plan_error is set (and nothing launched) when the call needs more CTAs than a grid has.
+cudaError_t launch_kv4_attention(const Kv4Attention& c, int* plan_error);
+
+// Sampling (rtd_sample.cu); null filters are off.
+constexpr int64_t kSampleMaxVocab = 1 << 19;  // 2^44-scaled weights sum below 2^63
+cudaError_t launch_sample(const void* x, int dt, int64_t ldx, int64_t T, int64_t V, const float* temperature,
+                          const int* top_k, const float* top_p, const float* min_p, const float* u, int* ids,
+                          cudaStream_t st);
+
 // y[m, n] = bias[n] (or 0) for every row m < M: the K = 0 case of a linear.
 cudaError_t launch_fill_rows(const float* bias, void* y, int y_dtype, int64_t ldy, int64_t M, int64_t N,
                              cudaStream_t st);
