@@ -64,7 +64,6 @@ constexpr size_t kWorkspaceBytes = 64ull << 20;  // activation staging (GEMV pre
 // the four-column GEMV pass is slower than one TN = 16 GEMM tile from M = 4 on, and
 // faster up to M = 3
 constexpr int64_t kGemmMinTokens = 4;
-constexpr size_t kAttnCountBytes = 64 << 10;
 constexpr size_t kAmaxBytes = 64;  // rtd_ctx::amax: 4 keys of 8 bytes, the count, padding
 
 thread_local std::string g_thread_err;
@@ -161,8 +160,8 @@ rtd_status rtd_init(int device, rtd_ctx** out) {
       (e = cudaMalloc(&c->status, sizeof(int))) != cudaSuccess ||
       (e = cudaMemset(c->status, 0, sizeof(int))) != cudaSuccess ||
       (e = cudaMalloc(&c->amax, kAmaxBytes)) != cudaSuccess || (e = cudaMemset(c->amax, 0, kAmaxBytes)) != cudaSuccess ||
-      (e = cudaMalloc(&c->attn_count, kAttnCountBytes)) != cudaSuccess ||
-      (e = cudaMemset(c->attn_count, 0, kAttnCountBytes)) != cudaSuccess) {
+      (e = cudaMalloc(&c->attn_count, rtd::kv4_attention_count_bytes(c->sm_count))) != cudaSuccess ||
+      (e = cudaMemset(c->attn_count, 0, rtd::kv4_attention_count_bytes(c->sm_count))) != cudaSuccess) {
     cudaFree(c->ws);
     cudaFree(c->status);
     cudaFree(c->amax);
@@ -830,14 +829,12 @@ rtd_status rtd_attention_kv4(rtd_ctx* ctx, const void* q, uint32_t q_dtype, int6
   if (max_q <= 0) return fail(ctx, RTD_ERR_SHAPE, "%s: max_q %d", who, max_q);
   rtd::Kv4Attention c{q, (int)q_dtype, ldq, T, n_head, n_kv, head_dim, scale, q_start, ctx_len, S, block_table,
                       max_blocks, max_q, max_ctx, static_cast<const uint8_t*>(pages), num_blocks, o, (int)o_dtype, ldo,
-                      ctx->ws, ctx->ws_bytes, ctx->attn_count, (int64_t)(kAttnCountBytes / sizeof(unsigned)),
-                      ctx->status, ctx->sm_count, (cudaStream_t)stream};
+                      ctx->ws, ctx->attn_count, ctx->status, ctx->sm_count, (cudaStream_t)stream};
+  if (rtd::kv4_attention_ws_bytes(ctx->sm_count) > ctx->ws_bytes)
+    return fail(ctx, RTD_ERR_WORKSPACE, "%s: the partial states do not fit the context workspace", who);
   DeviceGuard g(ctx->device);
   if (g.err != cudaSuccess) return cuda_fail(ctx, g.err, who);
-  int plan_err = 0;
-  cudaError_t e = rtd::launch_kv4_attention(c, &plan_err);
-  if (plan_err)
-    return fail(ctx, RTD_ERR_SHAPE, "%s: %d sequences x %d kv heads x %d queries are more than a grid holds", who, S, n_kv, max_q);
+  cudaError_t e = rtd::launch_kv4_attention(c);
   return e == cudaSuccess ? RTD_OK : cuda_fail(ctx, e, who);
 }
 

@@ -188,16 +188,15 @@ struct Kv4Attention {
   void* o;
   int o_dtype;
   int64_t ldo;
-  float* ws;          // the chunks' partial states
-  size_t ws_bytes;
-  unsigned* count;    // CTAs done per tile, zero between calls (the last one clears its word)
-  int64_t count_words;
+  float* ws;          // partial states: kv4_attention_ws_bytes
+  unsigned* count;    // kv4_attention_count_bytes, zero between calls (a word's last user clears it)
   int* status;
   int sm_count;
   cudaStream_t stream;
 };
-// *plan_error is set (and nothing launched) when the call needs more CTAs than a grid has.
-cudaError_t launch_kv4_attention(const Kv4Attention& c, int* plan_error);
+cudaError_t launch_kv4_attention(const Kv4Attention& c);
+size_t kv4_attention_ws_bytes(int sm_count);
+size_t kv4_attention_count_bytes(int sm_count);
 
 // Sampling (rtd_sample.cu); null filters are off.
 constexpr int64_t kSampleMaxVocab = 1 << 19;  // 2^44-scaled weights sum below 2^63

@@ -25,6 +25,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "rtd_common.cuh"
@@ -383,34 +384,40 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const int* slots, int64_t
 }
 
 // ------------------------------------------------------------------ attention
-// CTA (sequence s, kv head, tile of 8 rows, chunk of keys); row = token * G + head of the
-// group.  Each of its four warps takes every fourth page of the chunk through its own
-// ring of bulk copies, with its own running softmax; the warps' states join in shared
-// memory, the chunks' in the workspace (the last CTA of a tile joins them in chunk order,
-// so the order of arrival changes nothing).
+// Work: a unit is (sequence s, kv head, tile of 8 rows; row = token * G + head of the
+// group), its cost the pages of its keys.  The units' pages form one line, which the
+// resident CTAs share evenly, whatever the lengths; a unit that crosses a border is joined
+// from its CTAs' partial states by the last of them, in CTA order, so equal calls give
+// equal bits.  Each CTA finds its place from the lengths (S loads and a scan).  Within a
+// CTA every fourth page goes to a warp, which streams it through its own ring of bulk
+// copies and keeps its own running softmax; the warps' states join in shared memory.
 //
 // The products run on the tensor cores on the codes themselves, and step and minimum are
-// applied to the 32-bit sums of each group:  q.k = sum_g d_g (q_g . c_g) + m_g sum(q_g).
-// A nibble masked into an f16 pair under the exponent of 1024 is 1024 + c (or 1024 + 16 c),
-// and one packed fma makes it c, exactly: a word of eight codes becomes four operand
-// registers with four masks, one shift and four fmas.  (Left as the subnormal c * 2^-24
-// the fma would be saved, but the tensor cores align a subnormal's product as if its
-// leading zeros counted: measured 2e-5 of the output against 64 bits.)  V takes c - 8, so
-// that a long mean of values near zero is a sum of both signs and not a difference of two
-// large ones; sum_j p_j (m_jg + 8 d_jg) is added in the end.
-// Rows 0..7 of the 16-row MMA hold the queries' f16 heads, rows 8..15 the remainders, so
-// that a query enters with 22 bits; likewise p * d_g for V.  Queries are scaled by a power
-// of two per row, and p by 2^8, to keep both parts inside f16's range.
+// applied to the 32-bit sums of each group:  q.k = sum_g d_g (q_g . c_g) + m_g sum(q_g),
+// the minima's part as one more MMA over the groups.  For V the weights p * d_g multiply
+// the codes, and one MMA of p with the headers gives sum p m_g and sum p d_g.
+//
+// EXACT (f32 outputs): rows 0..7 of the 16-row MMA hold the f16 heads of q and p d, rows
+// 8..15 the remainders, so that both enter with 22 bits (p d is split by an exact fma).  A
+// nibble masked into an f16 pair under the exponent of 1024 is 1024 + c (or 1024 + 16 c)
+// and one packed addition makes it c (16 c, against a 16th of the query), exactly; V takes
+// c - 8, so that a long mean of values near zero is a sum of both signs and not a
+// difference of two large ones.
+// Otherwise (16-bit outputs): the rows enter rounded to 11 bits and the nibble stays the
+// f16 subnormal c * 2^-24, which saves the addition; the tensor cores align a subnormal's
+// product as if its leading zeros counted, which costs 2e-5 of the output.
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kRows = 8;
-constexpr float kHeadroom = 8.0f;  // p = 2^(x - max + 8) right after the maximum is set ...
-constexpr float kGrowth = 12.0f;   // ... and the maximum stays until a score would pass 2^12
+constexpr int kCtasPerSm = 3;
+constexpr int kMaxCtas = 512;
+constexpr int kUnitCost = 8;  // what a unit costs beside its pages (queries, joins), in pages
 
 struct Kv4AttnArgs {
   const void* q;
   int q_dtype;
+  int q_wide;  // f32 rows on 16-byte boundaries
   int64_t ldq;
   int T, n_head, n_kv;
   float scale;
@@ -423,10 +430,11 @@ struct Kv4AttnArgs {
   int num_blocks;
   void* o;
   int o_dtype;
+  int o_wide;       // f32 rows on 16-byte boundaries
   int64_t ldo;
-  int tiles, chunk, chunks;  // 8-row tiles a sequence, keys a chunk, chunks a tile
-  float* part;               // [S][n_kv][tiles][chunks][8][D + 2]
-  unsigned* count;           // [S][n_kv][tiles], zero between calls
+  int min_share;    // pages a CTA takes at least
+  float* part;      // [CTA][2][8 (D + 2)]: the units begun before it, and left open by it
+  unsigned* count;  // [CTA]: parts done of the unit it leaves open, zero between calls
   int* status;
 };
 
@@ -437,385 +445,689 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // |e| <= 126
 
-// Nibbles 0 and 4 (odd = false) or 1 and 5 (odd = true) of w as the f16 pair c - S.
-template <int S, bool odd>
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unf2(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ __half2 as_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// Nibbles 0 and 4 (ODD = false) or 1 and 5 of w as an f16 pair, odd ones times 16: c - S
+// when EXACT, else the subnormals c * 2^-24.
+template <bool EXACT, int S, bool ODD>
 __device__ __forceinline__ uint32_t codes(uint32_t w) {
-  const uint32_t b = lop_and_or(w, odd ? 0x00F000F0u : 0x000F000Fu, 0x64006400u);
-  const __half2 h = *reinterpret_cast<const __half2*>(&b);
-  const __half2 r = odd ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-64.0f - S))
-                        : __hadd2(h, __float2half2_rn(-1024.0f - S));
-  return *reinterpret_cast<const uint32_t*>(&r);
+  constexpr uint32_t mask = ODD ? 0x00F000F0u : 0x000F000Fu;
+  if constexpr (!EXACT) return w & mask;
+  const __half2 h = as_h2(lop_and_or(w, mask, 0x64006400u));
+  return as_u32(__hadd2(h, __float2half2_rn(ODD ? -1024.0f - 16 * S : -1024.0f - S)));
 }
 
+// Shared memory by 32-bit address: through a generic pointer every load would pay for the
+// address space.  Volatile, since bulk copies change what lies there.
+__device__ __forceinline__ void lds(uint32_t at, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
+}
+__device__ __forceinline__ void lds(uint32_t at, uint32_t (&v)[2]) {
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
+}
+__device__ __forceinline__ uint32_t lds(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_half(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+  return v;
+}
+// NG words of a row.
 template <int NG>
-__global__ void __launch_bounds__(kAttnThreads) kv4_attn_kernel(const Kv4AttnArgs a) {
+__device__ __forceinline__ void lds_row(uint32_t at, uint32_t (&v)[NG]) {
+  if constexpr (NG == 4 || NG == 2) {
+    lds(at, v);
+  } else {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) v[g] = lds(at + 4 * g);
+  }
+}
+// D = A B (+ C), m16n8k16, f16 in, f32 out.
+__device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The line of work: this CTA's range of it and where that begins.
+struct Place {
+  int64_t total, share;
+  int64_t pos, end;  // this CTA's pages
+  int s;             // the sequence of the first, and
+  int64_t off;       // its place among that sequence's pages
+};
+
+template <int NG, bool EXACT>
+struct Attn {
+  static constexpr int D = 32 * NG, PB = 20 * D;
+  static constexpr int kPitch = D + 4;                          // a row of a warp's state in the join buffer
+  static constexpr int kState = kRows * kPitch + 2 * kRows;     // the rows, their maxima and denominators
+  static constexpr int kPart = kRows * (D + 2);
+  static constexpr int kJoinFloats = kAttnWarps * kState > kMaxCtas * kRows ? kAttnWarps * kState : kMaxCtas * kRows;
+  static constexpr int kJoinBytes = (kJoinFloats + 2 * kAttnWarps * kRows + 4) * 4;
+  static constexpr int kSmem = kAttnWarps * kStages * PB + kJoinBytes + NG * 1024;
+  const Kv4AttnArgs& a;
+  uint8_t* ring;      // this warp's pages
+  uint32_t ring32;
+  uint64_t* bars;     // and their barriers
+  float* join;        // the warps' states, then the parts' weights
+  uint32_t qfrag;     // this lane's query fragments, [group][k step][lane][16 bytes]
+  int G, lane, warp;
+  unsigned get = 0, phase = 0;  // the ring's next page to use, and its parity
+  unsigned put_at = 0;          // the ring's next page to ask for
+
+  // A stretch of one unit: what its sequence is, and this warp's pages in it.
+  struct Seg {
+    int s, qs, nq, ctx, kvh, tile;
+    int cost;     // the unit's length on the line: kUnitCost + its pages
+    int off, n;   // the stretch on it
+    int first, mine;  // this warp's first page, and how many
+    const int* table;
+    int ids;      // block ids of 32 of them, a lane each
+    bool bad;
+  };
+
+  __device__ int seq_info(int s, int& qs, int& nq, int& ctx, bool tell) const {
+    qs = __ldg(a.q_start + s);
+    nq = __ldg(a.q_start + s + 1) - qs;
+    ctx = __ldg(a.ctx_len + s);
+    bool bad = qs < 0 || nq < 0 || (int64_t)qs + nq > a.T || nq > a.max_q;
+    if (bad) nq = 0;
+    if (ctx > a.max_ctx) {
+      bad |= nq > 0;
+      ctx = 0;
+    }
+    ctx = max(ctx, 0);
+    if (bad && tell) raise_status(a.status, kDevCache);
+    return kUnitCost + (ctx + kTok - 1) / kTok;
+  }
+
+  // keys that a row of the sequence sees: those before and at its position
+  __device__ int seen(const Seg& g, int row) const { return max(0, g.ctx - g.nq + row / G + 1); }
+
+  __device__ void issue(Seg& g, int j) {  // ask for this warp's j-th page
+    if (j >= g.mine) return;
+    if ((j & 31) == 0) {
+      g.ids = 0;
+      if (j + lane < g.mine) {
+        g.ids = __ldg(g.table + (j + lane) * kAttnWarps);
+        if ((unsigned)g.ids >= (unsigned)a.num_blocks) {
+          g.bad = true;
+          g.ids = 0;
+        }
+      }
+    }
+    const int blk = __shfl_sync(0xffffffffu, g.ids, j & 31);
+    if (lane == 0) {
+      mbar_arrive_expect_tx(bars + put_at, PB);
+      bulk_g2s(ring + put_at * PB, a.pages + ((int64_t)blk * a.n_kv + g.kvh) * PB, PB, bars + put_at);
+    }
+    if (++put_at == kStages) put_at = 0;
+  }
+
+  // Sets up pages [off, off + n) of a unit's line and asks for this warp's first ones.
+  __device__ void begin(Seg& g) {
+    const int row0 = g.tile * kRows, rows = g.nq * G;
+    const int need = (seen(g, min(row0 + kRows, rows) - 1) + kTok - 1) / kTok;
+    g.first = max(0, g.off - kUnitCost) + warp;
+    const int last = min(g.off + g.n - kUnitCost, need);
+    g.mine = last > g.first ? (last - g.first + kAttnWarps - 1) / kAttnWarps : 0;
+    g.table = a.table + (int64_t)g.s * a.max_blocks + g.first;
+    g.bad = false;
+    for (int j = 0; j < kStages; ++j) issue(g, j);
+  }
+
+  __device__ void run(Place& w) {
+    Seg g;
+    g.s = w.s;
+    g.cost = seq_info(g.s, g.qs, g.nq, g.ctx, false);
+    int tiles = (g.nq * G + kRows - 1) / kRows;
+    int64_t unit = w.off / g.cost;  // within the sequence: kv head * tiles + tile
+    g.off = (int)(w.off - unit * g.cost);
+    auto locate = [&](Seg& g) {
+      while (unit >= (int64_t)a.n_kv * tiles) {  // on to the next sequence with queries
+        unit = 0;
+        ++g.s;
+        g.cost = seq_info(g.s, g.qs, g.nq, g.ctx, false);
+        tiles = (g.nq * G + kRows - 1) / kRows;
+      }
+      g.kvh = (int)(unit / tiles);
+      g.tile = (int)(unit - (int64_t)g.kvh * tiles);
+      g.n = (int)min((int64_t)(g.cost - g.off), w.end - w.pos);
+    };
+    locate(g);
+    begin(g);
+    for (;;) {
+      const Seg done = g;
+      const int64_t at = w.pos - g.off;  // the unit's place on the line
+      float M, l, o[NG][4][4], z[4];
+      pages(g, M, l, o, z);
+      const bool bad = g.bad;
+      w.pos += g.n;
+      const bool more = w.pos < w.end;
+      if (more) {  // the next stretch's pages are on their way while this one's warps join
+        g.off = 0;
+        ++unit;
+        locate(g);
+        begin(g);
+      }
+      finish(w, done, at, bad, M, l, o, z);
+      if (!more) break;
+    }
+  }
+
+  // This warp's pages of the stretch: per row the running maximum M and sum l, and in
+  // fragments the products o and the header sums z.
+  __device__ void pages(Seg& sg, float& M, float& l, float (&o)[NG][4][4], float (&z)[4]) {
+    const int qs = sg.qs, kvh = sg.kvh, mine = sg.mine, first = sg.first;
+    const int row0 = sg.tile * kRows, rows = sg.nq * G;
+    const int least = seen(sg, row0), most = seen(sg, min(row0 + kRows, rows) - 1);
+    // ---- queries: lane (row r, quad lane i) holds dims 8 i .. 8 i + 7 of every group
+    const int r = lane >> 2, qi = lane & 3;
+    const int row = row0 + r;
+    const bool live = row < rows;
+    const int limit = live ? seen(sg, row) : most;
+    uint32_t qm[2];
+    float rowmul;
+    {
+      float x[NG][8], qsum[NG];
+      const int64_t base = live ? (int64_t)(qs + row / G) * a.ldq + (int64_t)(kvh * G + row % G) * D : 0;
+      float mx = 0.0f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float sum = 0.0f;
+        const int64_t at = base + 32 * g + 8 * qi;
+        if (a.q_wide) {
+          *reinterpret_cast<float4*>(x[g]) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at));
+          *reinterpret_cast<float4*>(x[g] + 4) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at + 4));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[g][e] = load_as_f32(a.q, a.q_dtype, at + e);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = live ? x[g][e] * a.scale * 1.4426950408889634f : 0.0f;
+          x[g][e] = v;
+          sum += v;
+          mx = fmaxf(mx, fabsf(v));
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        qsum[g] = sum;
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // 2^k brings the row's largest into [2^6, 2^7): the group sums fit f16 too
+      int k = 0;
+      if (mx > 0.0f && mx < INFINITY) k = max(-90, min(90, 6 - ilogbf(mx)));
+      const float up = pow2(k);
+      rowmul = pow2(-k);
+      auto split = [](float v0, float v1, uint32_t& hi, uint32_t& lo) {
+        const __half2 h = __floats2half2_rn(v0, v1);
+        const float2 f = __half22float2(h);
+        hi = as_u32(h);
+        lo = as_u32(__floats2half2_rn(v0 - f.x, v1 - f.y));
+      };
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          uint32_t frag[4];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int e = 2 * st + b;  // nibbles e and e + 4; odd ones carry a factor 16
+            const float f = b ? up * 0.0625f : up;
+            split(x[g][e] * f, x[g][e + 4] * f, frag[2 * b], frag[2 * b + 1]);
+          }
+          // every warp has the same queries and writes the same words
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(qfrag + (g * 2 + st) * 512), "r"(frag[0]), "r"(frag[1]),
+                       "r"(frag[2]), "r"(frag[3])
+                       : "memory");
+        }
+      // the sums of groups 2 i and 2 i + 1, against the minima
+      float q0 = 0.0f, q1 = 0.0f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+        if (g / 2 == qi) {
+          if (g & 1)
+            q1 = qsum[g] * up;
+          else
+            q0 = qsum[g] * up;
+        }
+      split(q0, q1, qm[0], qm[1]);
+    }
+
+    const int kt = ((r & 1) << 2) | (r >> 1);  // token of S column r: columns 2 i, 2 i + 1 are tokens i, i + 4
+    // p = 2^(x - max + headroom) right after a maximum is set, which stays until a score
+    // would pass 2^growth; if p d left f16's range after all (a step above 16), the pages
+    // are read once more with p at most 1
+    for (int attempt = 0;; ++attempt) {
+      const float headroom = attempt ? 0.0f : 8.0f, growth = attempt ? 0.0f : 12.0f;
+      M = -1e30f;
+      l = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) z[c] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[g][p][c] = 0.0f;
+      for (int j = 0; j < mine; ++j) {
+        mbar_wait_bounded(bars + get, phase, a.status);
+        const uint32_t page = ring32 + get * PB;
+        if (++get == kStages) {
+          get = 0;
+          phase ^= 1;
+        }
+        const int key = (first + j * kAttnWarps) * kTok;
+        const bool partial = key + kTok > least;
+        // ---- scores
+        uint64_t x2[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t kw[NG], h0[NG], h1[NG], hm[2] = {0, 0};
+          const uint32_t ph = page + 8 * D + 8 * u * (4 * NG);
+          lds_row<NG>(page + (8 * u + kt) * (D / 2) + qi * (4 * NG), kw);
+          lds_row<NG>(ph + qi * (4 * NG), h0);
+          lds_row<NG>(ph + (4 + qi) * (4 * NG), h1);
+          if constexpr (NG == 4) {
+            lds(ph + kt * 16 + 8 * (qi & 1), hm);
+          } else {
+            if (2 * qi < NG) hm[0] = lds(ph + kt * (4 * NG) + 8 * qi);
+            if (2 * qi + 1 < NG) hm[1] = lds(ph + kt * (4 * NG) + 8 * qi + 4);
+          }
+          float acc[4];
+          uint32_t bm = prmt(hm[0], hm[1], 0x7632u);
+          if (qi >= 2) bm = 0;
+          mma0(acc, qm[0], EXACT ? qm[1] : 0u, 0u, 0u, bm, 0u);
+          x2[u] = EXACT ? add2(f2(acc[0], acc[1]), f2(acc[2], acc[3])) : f2(acc[0], acc[1]);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const uint32_t hw = kw[g] >> 8;
+            float e[4];
+            uint32_t qa[4];
+            lds(qfrag + g * 1024, qa);
+            mma0(e, qa[0], EXACT ? qa[1] : 0u, qa[2], EXACT ? qa[3] : 0u, codes<EXACT, 0, false>(kw[g]), codes<EXACT, 0, true>(kw[g]));
+            lds(qfrag + g * 1024 + 512, qa);
+            mma(e, qa[0], EXACT ? qa[1] : 0u, qa[2], EXACT ? qa[3] : 0u, codes<EXACT, 0, false>(hw), codes<EXACT, 0, true>(hw));
+            float d0 = __low2float(as_h2(h0[g])), d1 = __low2float(as_h2(h1[g]));
+            uint64_t sum = f2(e[0], e[1]);
+            if constexpr (EXACT) {
+              sum = add2(sum, f2(e[2], e[3]));
+            } else {
+              d0 *= 16777216.0f;  // the codes' 2^-24
+              d1 *= 16777216.0f;
+            }
+            x2[u] = fma2(f2(d0, d1), sum, x2[u]);
+          }
+        }
+        float x[2][2];
+        *reinterpret_cast<float2*>(x[0]) = unf2(x2[0]);
+        *reinterpret_cast<float2*>(x[1]) = unf2(x2[1]);
+        const uint32_t vh = page + 18 * D;
+        if (partial) {
+          // Keys that a row does not see weigh nothing, whatever they hold: scores -inf, and
+          // V headers that are not finite zeroed, since 0 * NaN would reach every row of the
+          // MMA; a row that does see such a header gets its group's NaN here.
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              if (key + 8 * u + 4 * c + qi >= limit) x[u][c] = -INFINITY;
+          uint64_t nan_at = 0;
+#pragma unroll
+          for (int i = 0; i < (16 * NG + 31) / 32; ++i) {
+            const int at = 32 * i + lane;
+            bool no = false;
+            if (at < 16 * NG) {
+              const uint32_t h = lds(vh + 4 * at);
+              no = (h & 0x7c00u) == 0x7c00u || (h & 0x7c000000u) == 0x7c000000u;
+              if (no) asm volatile("st.shared.u32 [%0], %1;" ::"r"(vh + 4 * at), "r"(0u) : "memory");
+            }
+            nan_at |= (uint64_t)__ballot_sync(0xffffffffu, no) << (32 * i);
+          }
+          if (nan_at) {
+            const int cnt = max(0, min(kTok, limit - key));
+            for (int t = 0; t < cnt; ++t)
+#pragma unroll
+              for (int g = 0; g < NG; ++g)
+                if ((nan_at >> (t * NG + g)) & 1)
+#pragma unroll
+                  for (int p = 0; p < 4; ++p) o[g][p][0] = o[g][p][1] = NAN;
+          }
+          // the next bulk copy into this page follows these stores
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        // ---- running softmax
+        float mx = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])) * rowmul;
+        if (__any_sync(0xffffffffu, mx > M + growth)) {
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          if (mx > M + growth) {
+            const float to = mx - headroom, f = ex2(M - to);
+            M = to;
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) z[c] *= f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[g][p][c] *= f;
+          }
+        }
+        uint32_t ph[2], pl[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float p0 = ex2(fmaf(x[u][0], rowmul, -M)), p1 = ex2(fmaf(x[u][1], rowmul, -M));
+          l += p0 + p1;
+          const __half2 h = __floats2half2_rn(p0, p1);
+          ph[u] = as_u32(h);
+          if constexpr (EXACT) {
+            const float2 f = __half22float2(h);
+            pl[u] = as_u32(__floats2half2_rn(p0 - f.x, p1 - f.y));
+          } else {
+            pl[u] = 0;
+          }
+        }
+        // ---- sums of p times the minima (columns 0..3) and the steps (columns 4..7)
+        {
+          const int g = min(r & 3, NG - 1);
+          const uint32_t sel = r < 4 ? 0x7632u : 0x5410u;
+          const uint32_t at = vh + 4 * (qi * NG + g);
+          const uint32_t b0 = prmt(lds(at), lds(at + 16 * NG), sel), b1 = prmt(lds(at + 32 * NG), lds(at + 48 * NG), sel);
+          mma(z, ph[0], pl[0], ph[1], pl[1], b0, b1);
+        }
+        // ---- O += (p d) C: pairs of tokens (i, i + 4) and (i + 8, i + 12)
+        uint32_t vd[4][NG], vw[4][(NG + 1) / 2];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t vr = page + 10 * D + (4 * c + qi) * (D / 2);
+          lds_row<NG>(vh + (4 * c + qi) * (4 * NG), vd[c]);
+          if constexpr (NG == 4) {
+            lds(vr + (((2 * r) ^ (8 * (qi >> 1))) << 2), vw[c]);
+          } else {
+            if constexpr (NG >= 2) vw[c][0] = lds(vr + 4 * r);
+            if constexpr (NG & 1) vw[c][NG / 2] = lds_half(vr + ((NG - 1) * 8 + r) * 2);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          uint32_t hi[2], lo[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const __half2 d = as_h2(prmt(vd[2 * u][g], vd[2 * u + 1][g], 0x5410u));
+            const __half2 p = as_h2(ph[u]), h = __hmul2(p, d);
+            hi[u] = as_u32(h);
+            lo[u] = EXACT ? as_u32(__hfma2(as_h2(pl[u]), d, __hfma2(p, d, __hneg2(h)))) : 0u;
+          }
+          const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+          const uint32_t b0 = prmt(vw[0][g / 2], vw[1][g / 2], sel), b1 = prmt(vw[2][g / 2], vw[3][g / 2], sel);
+          mma(o[g][0], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, false>(b0), codes<EXACT, 8, false>(b1));
+          mma(o[g][1], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, true>(b0), codes<EXACT, 8, true>(b1));
+          mma(o[g][2], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, false>(b0 >> 8), codes<EXACT, 8, false>(b1 >> 8));
+          mma(o[g][3], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, true>(b0 >> 8), codes<EXACT, 8, true>(b1 >> 8));
+        }
+        __syncwarp();
+        issue(sg, j + kStages);
+      }
+      if (attempt || mine == 0) break;
+      float probe = 0.0f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) probe = fmaf(o[g][p][c], 0.0f, probe);
+      if (!__any_sync(0xffffffffu, probe != 0.0f)) break;  // NaN where anything was not finite
+      for (int j = 0; j < kStages; ++j) issue(sg, j);
+    }
+  }
+
+  // Joins the warps' states and, where the unit goes on in other CTAs, the CTAs'.
+  __device__ void finish(const Place& w, const Seg& sg, int64_t begin, bool bad, float M, float l, const float (&o)[NG][4][4],
+                         const float (&z)[4]) {
+    const int r = lane >> 2, qi = lane & 3;
+    const int qs = sg.qs, kvh = sg.kvh, row0 = sg.tile * kRows, rows = sg.nq * G;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (__any_sync(0xffffffffu, bad)) {  // a block id outside the pool: no number stands for these rows
+      if (lane == 0) raise_status(a.status, kDevCache);
+      l = NAN;
+    }
+    {
+      float* out = join + warp * kState + r * kPitch + 8 * qi;
+      const float z0 = z[0] + z[2], z1 = z[1] + z[3];  // quad lanes 0, 1: minima; 2, 3: steps
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int from = (lane & ~3) + g / 2;
+        const float zm = __shfl_sync(0xffffffffu, (g & 1) ? z1 : z0, from);
+        const float zd = __shfl_sync(0xffffffffu, (g & 1) ? z1 : z0, from + 2);
+        const float zz = EXACT ? fmaf(8.0f, zd, zm) : zm;
+        float v[8];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const float f = (EXACT ? 1.0f : 16777216.0f) * ((p & 1) ? 0.0625f : 1.0f);  // the odd nibbles' 16
+          v[p] = fmaf(o[g][p][0] + o[g][p][2], f, zz);
+          v[4 + p] = fmaf(o[g][p][1] + o[g][p][3], f, zz);
+        }
+        *reinterpret_cast<float4*>(out + 32 * g) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(out + 32 * g + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      }
+      if (qi == 0) {
+        join[warp * kState + kRows * kPitch + r] = M;
+        join[warp * kState + kRows * kPitch + kRows + r] = l;
+      }
+    }
+    __syncthreads();
+    const int tid = threadIdx.x;
+    const int cta = blockIdx.x;
+    const int c0 = (int)(begin / w.share), c1 = (int)((begin + sg.cost - 1) / w.share);
+    // a part: [8][D] sums, [8] maxima, [8] denominators
+    auto part = [&](int c) { return a.part + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * kPart; };
+    auto put = [&](int rr, int d, float4 v, float ls) {
+      const int rw = row0 + rr;
+      if (rw >= rows) return;
+      const float f = ls == 0.0f ? 0.0f : 1.0f / ls;
+      if (ls == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const int64_t at = (int64_t)(qs + rw / G) * a.ldo + (int64_t)(kvh * G + rw % G) * D + d;
+      if (a.o_wide && a.o_dtype == 0) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+      } else {
+        store_from_f32(a.o, a.o_dtype, at, v.x * f);
+        store_from_f32(a.o, a.o_dtype, at + 1, v.y * f);
+        store_from_f32(a.o, a.o_dtype, at + 2, v.z * f);
+        store_from_f32(a.o, a.o_dtype, at + 3, v.w * f);
+      }
+    };
+    for (int e = tid; e < kRows * D / 4; e += kAttnThreads) {
+      const int rr = e / (D / 4), d = 4 * (e - rr * (D / 4));
+      const float* ml = join + kRows * kPitch + rr;
+      float m = ml[0];
+#pragma unroll
+      for (int k = 1; k < kAttnWarps; ++k) m = fmaxf(m, ml[k * kState]);
+      float ls = 0.0f;
+      float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < kAttnWarps; ++k) {
+        const float f = ex2(ml[k * kState] - m);
+        const float4 v = *reinterpret_cast<const float4*>(join + k * kState + rr * kPitch + d);
+        ls = fmaf(ml[k * kState + kRows], f, ls);
+        os = make_float4(fmaf(v.x, f, os.x), fmaf(v.y, f, os.y), fmaf(v.z, f, os.z), fmaf(v.w, f, os.w));
+      }
+      if (c0 == c1) {
+        put(rr, d, os, ls);
+      } else {
+        float* p = part(cta);
+        *reinterpret_cast<float4*>(p + rr * D + d) = os;
+        if (d == 0) {
+          p[kRows * D + rr] = m;
+          p[kRows * D + kRows + rr] = ls;
+        }
+      }
+    }
+    if (c0 != c1) {  // the last CTA of the unit joins its parts, in CTA order
+      float* red = join + kJoinFloats;  // [2][4 warps][8], and the flag
+      int* last = reinterpret_cast<int*>(red + 2 * kAttnWarps * kRows);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        *last = atomicAdd(a.count + c0, 1u) == (unsigned)(c1 - c0);
+        if (*last) a.count[c0] = 0;
+      }
+      __syncthreads();
+      if (*last) {
+        __threadfence();
+        // the parts' weights 2^(m_c - m), [c][8] in the join buffer: a thread takes a row
+        // and every 16th part
+        const int rr = tid & 7;
+        float m = -1e30f, ls = 0.0f;
+        for (int c = c0 + (tid >> 3); c <= c1; c += kAttnThreads / 8) {
+          const float v = __ldcg(part(c) + kRows * D + rr);
+          join[(c - c0) * kRows + rr] = v;
+          m = fmaxf(m, v);
+        }
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if (lane < kRows) red[warp * kRows + rr] = m;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kAttnWarps; ++k) m = fmaxf(m, red[k * kRows + rr]);
+        for (int c = c0 + (tid >> 3); c <= c1; c += kAttnThreads / 8) {
+          const float f = ex2(join[(c - c0) * kRows + rr] - m);
+          join[(c - c0) * kRows + rr] = f;
+          ls = fmaf(__ldcg(part(c) + kRows * D + kRows + rr), f, ls);
+        }
+        ls += __shfl_xor_sync(0xffffffffu, ls, 8);
+        ls += __shfl_xor_sync(0xffffffffu, ls, 16);
+        if (lane < kRows) red[(kAttnWarps + warp) * kRows + rr] = ls;
+        __syncthreads();
+        for (int e = tid; e < kRows * D / 4; e += kAttnThreads) {
+          const int er = e / (D / 4), d = 4 * (e - er * (D / 4));
+          float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+          for (int c = c0; c <= c1; ++c) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part(c) + er * D + d));
+            const float f = join[(c - c0) * kRows + er];
+            os = make_float4(fmaf(v.x, f, os.x), fmaf(v.y, f, os.y), fmaf(v.z, f, os.z), fmaf(v.w, f, os.w));
+          }
+          const float* lr = red + kAttnWarps * kRows + er;
+          put(er, d, os, (lr[0] + lr[kRows]) + (lr[2 * kRows] + lr[3 * kRows]));
+        }
+      }
+    }
+    __syncthreads();  // the join buffer is used again
+  }
+};
+
+template <int NG, bool EXACT>
+__global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) kv4_attn_kernel(const Kv4AttnArgs a) {
   constexpr int D = 32 * NG, PB = 20 * D;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kAttnWarps][kStages];
-  __shared__ int last;
-  const int G = a.n_head / a.n_kv;
-  // tile fastest: CTAs that read the same keys run together
-  unsigned bid = blockIdx.x;
-  const int tile = a.tiles - 1 - (int)(bid % a.tiles);  // later tiles see more keys: first
-  bid /= a.tiles;
-  const int chunk = (int)(bid % a.chunks);
-  bid /= a.chunks;
-  const int kvh = (int)(bid % a.n_kv), s = (int)(bid / a.n_kv);
+  __shared__ int64_t sums[kAttnWarps];
+  __shared__ Place place;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int qs = __ldg(a.q_start + s), nq = __ldg(a.q_start + s + 1) - qs;
-  int ctx = __ldg(a.ctx_len + s);
-  if (qs < 0 || nq < 0 || (int64_t)qs + nq > a.T || nq > a.max_q) {
-    if (tid == 0) raise_status(a.status, kDevCache);
-    return;
-  }
-  if (ctx > a.max_ctx) {
-    if (tid == 0) raise_status(a.status, kDevCache);
-    ctx = 0;
-  }
-  const int row0 = tile * kRows, rows = nq * G;
-  if (row0 >= rows) return;
-  // keys seen by a row: its position and before
-  auto seen = [&](int row) { return max(0, ctx - nq + row / G + 1); };
-  const int most = seen(min(row0 + kRows, rows) - 1);
-  const int active = max(1, (most + a.chunk - 1) / a.chunk);
-  if (chunk >= active) return;
-  const int key0 = chunk * a.chunk, key1 = min(most, key0 + a.chunk);
-  const int page0 = key0 / kTok, npages = (max(0, key1 - key0) + kTok - 1) / kTok;
-  const int mine = npages > warp ? (npages - warp + kAttnWarps - 1) / kAttnWarps : 0;
-
-  // ---- this warp's ring of pages
-  uint8_t* ring = smem + warp * (kStages * PB);
-  const int* table = a.table + (int64_t)s * a.max_blocks + page0 + warp;
-  bool bad = false;
-  int ids = 0;
-  auto load_ids = [&](int base) {
-    const int j = base + lane;
-    ids = 0;
-    if (j < mine) {
-      ids = __ldg(table + j * kAttnWarps);
-      if ((unsigned)ids >= (unsigned)a.num_blocks) {
-        bad = true;
-        ids = 0;
-      }
-    }
-  };
-  auto issue = [&](int j) {
-    if (j >= mine) return;
-    if ((j & 31) == 0) load_ids(j);
-    const int blk = __shfl_sync(0xffffffffu, ids, j & 31);
-    if (lane == 0) {
-      uint64_t* bar = &bars[warp][j % kStages];
-      mbar_arrive_expect_tx(bar, PB);
-      bulk_g2s(ring + (j % kStages) * PB, a.pages + ((int64_t)blk * a.n_kv + kvh) * PB, PB, bar);
-    }
-  };
+  Attn<NG, EXACT> at{a, smem + warp * (kStages * PB), smem_u32(smem + warp * (kStages * PB)), bars[warp], reinterpret_cast<float*>(smem + kAttnWarps * kStages * PB),
+                     smem_u32(smem + kAttnWarps * kStages * PB + Attn<NG, EXACT>::kJoinBytes) + 16 * lane,
+                     a.n_head / a.n_kv, lane, warp};
   if (lane == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(&bars[warp][i], 1);
     fence_mbar_init();
   }
-  __syncwarp();
-  for (int j = 0; j < kStages; ++j) issue(j);
-
-  // ---- queries: lane (row r, quad lane i) holds dims 8 i .. 8 i + 7 of every group
-  const int r = lane >> 2, qi = lane & 3;
-  const int row = row0 + r;
-  const bool live = row < rows;
-  const int limit = live ? min(seen(row), key1) : 0;
-  uint32_t qa[NG][2][4];
-  float qsum[NG], rowmul;
-  {
-    float x[NG][8];
-    const int64_t base = live ? (int64_t)(qs + row / G) * a.ldq + (int64_t)(kvh * G + row % G) * D : 0;
-    float mx = 0.0f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = live ? load_as_f32(a.q, a.q_dtype, base + 32 * g + 8 * qi + e) * a.scale * 1.4426950408889634f : 0.0f;
-        x[g][e] = v;
-        sum += v;
-        mx = fmaxf(mx, fabsf(v));
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      qsum[g] = sum;
-    }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    // 2^k brings the row's largest into [2^12, 2^13)
-    int k = 0;
-    if (mx > 0.0f && mx < INFINITY) k = max(-100, min(100, 12 - ilogbf(mx)));
-    const float up = pow2(k);
-    rowmul = pow2(-k);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      qsum[g] *= up;
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int e = 2 * st + b;  // nibbles e and e + 4
-          const float v0 = x[g][e] * up, v1 = x[g][e + 4] * up;
-          const __half2 hi = __floats2half2_rn(v0, v1);
-          const float2 hf = __half22float2(hi);
-          const __half2 lo = __floats2half2_rn(v0 - hf.x, v1 - hf.y);
-          qa[g][st][2 * b] = *reinterpret_cast<const uint32_t*>(&hi);
-          qa[g][st][2 * b + 1] = *reinterpret_cast<const uint32_t*>(&lo);
-        }
-    }
-  }
-
-  float M = -1e30f, l = 0.0f;
-  float z[NG], o[NG][4][4];
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    z[g] = 0.0f;
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[g][p][c] = 0.0f;
-  }
-  auto rescale = [&](float f) {
-    l *= f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      z[g] *= f;
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[g][p][c] *= f;
-    }
+  // ---- the line of work and this CTA's place on it
+  const int per = (a.S + kAttnThreads - 1) / kAttnThreads;
+  const int s0 = min(a.S, tid * per), s1 = min(a.S, s0 + per);
+  auto cost = [&](int s) -> int64_t {
+    int qs, nq, ctx;
+    const int unit = at.seq_info(s, qs, nq, ctx, blockIdx.x == 0);
+    return (int64_t)a.n_kv * ((nq * at.G + kRows - 1) / kRows) * unit;
   };
-
-  // ---- pages
-  const int kt = ((r & 1) << 2) | (r >> 1);  // token of S column r: columns 2 i, 2 i + 1 are tokens i, i + 4
-  for (int j = 0; j < mine; ++j) {
-    const int st = j % kStages;
-    mbar_wait_bounded(&bars[warp][st], (j / kStages) & 1, a.status);
-    const uint8_t* page = ring + st * PB;
-    const int key = key0 + (warp + j * kAttnWarps) * kTok;
-    float x[2][2];
+  int64_t mine = 0;
+  for (int s = s0; s < s1; ++s) mine += cost(s);
+  int64_t inc = mine;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      uint32_t w[NG], h0[NG], h1[NG];
-      const uint32_t* kw = reinterpret_cast<const uint32_t*>(page + (8 * u + kt) * (D / 2)) + qi * NG;
-      const uint32_t* kh = reinterpret_cast<const uint32_t*>(page + 8 * D) + (8 * u + qi) * NG;
-      if constexpr (NG == 4) {
-        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(kw);
-        *reinterpret_cast<uint4*>(h0) = *reinterpret_cast<const uint4*>(kh);
-        *reinterpret_cast<uint4*>(h1) = *reinterpret_cast<const uint4*>(kh + 4 * NG);
-      } else {
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          w[g] = kw[g];
-          h0[g] = kh[g];
-          h1[g] = kh[4 * NG + g];
-        }
-      }
-      x[u][0] = x[u][1] = 0.0f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint32_t hiw = w[g] >> 8;
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        mma_f16_acc(acc, qa[g][0][0], qa[g][0][1], qa[g][0][2], qa[g][0][3], codes<0, false>(w[g]),
-                    codes<0, true>(w[g]));
-        mma_f16_acc(acc, qa[g][1][0], qa[g][1][1], qa[g][1][2], qa[g][1][3], codes<0, false>(hiw),
-                    codes<0, true>(hiw));
-        const float2 d0 = __half22float2(*reinterpret_cast<__half2*>(&h0[g]));
-        const float2 d1 = __half22float2(*reinterpret_cast<__half2*>(&h1[g]));
-        x[u][0] = fmaf(d0.x, acc[0] + acc[2], fmaf(d0.y, qsum[g], x[u][0]));
-        x[u][1] = fmaf(d1.x, acc[1] + acc[3], fmaf(d1.y, qsum[g], x[u][1]));
-      }
-    }
-    bool vis[2][2];
-    float mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        vis[u][c] = key + 8 * u + 4 * c + qi < limit;
-        x[u][c] = vis[u][c] ? x[u][c] * rowmul : -INFINITY;
-        mx = fmaxf(mx, x[u][c]);
-      }
-    if (__any_sync(0xffffffffu, mx > M + kGrowth)) {
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      if (mx > M + kGrowth) {
-        const float to = mx - kHeadroom;
-        rescale(ex2(M - to));
-        M = to;
-      }
-    }
-    float p[2][2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) p[u][c] = ex2(x[u][c] - M);
-    // V headers of this lane's four tokens
-    float pd[NG][4], over = 0.0f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t* vh = reinterpret_cast<const uint32_t*>(page + 18 * D) + (8 * u + 4 * c + qi) * NG;
-        uint32_t h[NG];
-        if constexpr (NG == 4)
-          *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(vh);
-        else
-#pragma unroll
-          for (int g = 0; g < NG; ++g) h[g] = vh[g];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const float2 dm = __half22float2(*reinterpret_cast<__half2*>(&h[g]));
-          // a key that this row does not see may hold anything
-          pd[g][2 * u + c] = vis[u][c] ? p[u][c] * dm.x : 0.0f;
-          z[g] = vis[u][c] ? fmaf(p[u][c], dm.y, fmaf(8.0f, pd[g][2 * u + c], z[g])) : z[g];
-          over = fmaxf(over, pd[g][2 * u + c]);
-        }
-      }
-    l += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
-    if (__any_sync(0xffffffffu, over > 60000.0f)) {  // a step above 16: lower p until it fits f16
-      over = fmaxf(over, __shfl_xor_sync(0xffffffffu, over, 1));
-      over = fmaxf(over, __shfl_xor_sync(0xffffffffu, over, 2));
-      if (over > 60000.0f && over < INFINITY) {
-        const int e = ilogbf(over) - 13;
-        const float f = pow2(-e);
-        M += (float)e;
-        rescale(f);
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) pd[g][c] *= f;
-      }
-    }
-    // O += (p d) C: pairs of tokens (i, i + 4) and (i + 8, i + 12)
-    uint32_t v[4][(NG + 1) / 2];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint8_t* vr = page + 10 * D + (4 * c + qi) * (D / 2);
-      if constexpr (NG == 4) {
-        *reinterpret_cast<uint2*>(v[c]) = *reinterpret_cast<const uint2*>(vr + (((2 * r) ^ (8 * (qi >> 1))) << 2));
-      } else {
-        if constexpr (NG >= 2) v[c][0] = *reinterpret_cast<const uint32_t*>(vr + 4 * r);
-        if constexpr (NG & 1) v[c][NG / 2] = *reinterpret_cast<const uint16_t*>(vr + ((NG - 1) * 8 + r) * 2);
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const __half2 h0 = __floats2half2_rn(pd[g][0], pd[g][1]), h1 = __floats2half2_rn(pd[g][2], pd[g][3]);
-      const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-      const __half2 l0 = __floats2half2_rn(pd[g][0] - f0.x, pd[g][1] - f0.y);
-      const __half2 l1 = __floats2half2_rn(pd[g][2] - f1.x, pd[g][3] - f1.y);
-      const uint32_t a0 = *reinterpret_cast<const uint32_t*>(&h0), a1 = *reinterpret_cast<const uint32_t*>(&l0);
-      const uint32_t a2 = *reinterpret_cast<const uint32_t*>(&h1), a3 = *reinterpret_cast<const uint32_t*>(&l1);
-      const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
-      const uint32_t b0 = prmt(v[0][g / 2], v[1][g / 2], sel), b1 = prmt(v[2][g / 2], v[3][g / 2], sel);
-      mma_f16_acc(o[g][0], a0, a1, a2, a3, codes<8, false>(b0), codes<8, false>(b1));
-      mma_f16_acc(o[g][1], a0, a1, a2, a3, codes<8, true>(b0), codes<8, true>(b1));
-      mma_f16_acc(o[g][2], a0, a1, a2, a3, codes<8, false>(b0 >> 8), codes<8, false>(b1 >> 8));
-      mma_f16_acc(o[g][3], a0, a1, a2, a3, codes<8, true>(b0 >> 8), codes<8, true>(b1 >> 8));
-    }
-    __syncwarp();
-    issue(j + kStages);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
   }
-
-  // ---- join the warps (the ring's memory is free once every warp is done)
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
-  if (__any_sync(0xffffffffu, bad)) {  // a block id outside the pool: no number stands for these rows
-    if (lane == 0) raise_status(a.status, kDevCache);
-    l = NAN;
-  }
+  if (lane == 31) sums[warp] = inc;
   __syncthreads();
-  float* st = reinterpret_cast<float*>(smem);  // [warp][8][D + 2]
-  {
-    float* w = st + (warp * kRows + r) * (D + 2);
+  int64_t total = 0;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float zz = z[g];
-      zz += __shfl_xor_sync(0xffffffffu, zz, 1);
-      zz += __shfl_xor_sync(0xffffffffu, zz, 2);
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        w[32 * g + 8 * qi + p] = (o[g][p][0] + o[g][p][2]) + zz;
-        w[32 * g + 8 * qi + 4 + p] = (o[g][p][1] + o[g][p][3]) + zz;
+  for (int k = 0; k < kAttnWarps; ++k) {
+    if (k < warp) inc += sums[k];
+    total += sums[k];
+  }
+  const int64_t share = max((int64_t)a.min_share, (total + gridDim.x - 1) / gridDim.x);
+  const int64_t pos = share * blockIdx.x;
+  if (pos >= total) return;
+  int64_t before = inc - mine;
+  if (pos >= before && pos < inc)
+    for (int s = s0; s < s1; ++s) {
+      const int64_t c = cost(s);
+      if (pos < before + c) {
+        place = Place{total, share, pos, min(total, pos + share), s, pos - before};
+        break;
       }
+      before += c;
     }
-    if (qi == 0) {
-      w[D] = M;
-      w[D + 1] = l;
-    }
-  }
   __syncthreads();
-  const int64_t unit = ((int64_t)s * a.n_kv + kvh) * a.tiles + tile;
-  float* part = a.part + (unit * a.chunks + chunk) * (kRows * (D + 2));
-  auto put = [&](int rr, int d, float v) {
-    const int rw = row0 + rr;
-    if (rw < rows)
-      store_from_f32(a.o, a.o_dtype, (int64_t)(qs + rw / G) * a.ldo + (int64_t)(kvh * G + rw % G) * D + d, v);
-  };
-  for (int e = tid; e < kRows * D; e += kAttnThreads) {
-    const int rr = e / D, d = e - rr * D;
-    const float* w = st + rr * (D + 2);
-    constexpr int ws = kRows * (D + 2);
-    float m = w[D];
-#pragma unroll
-    for (int k = 1; k < kAttnWarps; ++k) m = fmaxf(m, w[k * ws + D]);
-    float ls = 0.0f, os = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kAttnWarps; ++k) {
-      const float f = ex2(w[k * ws + D] - m);
-      ls = fmaf(w[k * ws + D + 1], f, ls);
-      os = fmaf(w[k * ws + d], f, os);
-    }
-    if (active == 1) {
-      put(rr, d, ls == 0.0f ? 0.0f : os / ls);
-    } else {
-      part[rr * (D + 2) + d] = os;
-      if (d == 0) {
-        part[rr * (D + 2) + D] = m;
-        part[rr * (D + 2) + D + 1] = ls;
-      }
-    }
-  }
-  if (active == 1) return;
-  // ---- the last chunk of the tile joins them all, in chunk order
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    last = atomicAdd(a.count + unit, 1u) == (unsigned)active - 1u;
-    if (last) a.count[unit] = 0;
-  }
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  const float* all = a.part + unit * a.chunks * (kRows * (D + 2));
-  constexpr int cs = kRows * (D + 2);
-  for (int e = tid; e < kRows * D; e += kAttnThreads) {
-    const int rr = e / D, d = e - rr * D;
-    const float* w = all + rr * (D + 2);
-    float m = -1e30f;
-    for (int k = 0; k < active; ++k) m = fmaxf(m, __ldcg(w + (int64_t)k * cs + D));
-    float ls = 0.0f, os = 0.0f;
-    for (int k = 0; k < active; ++k) {
-      const float f = ex2(__ldcg(w + (int64_t)k * cs + D) - m);
-      ls = fmaf(__ldcg(w + (int64_t)k * cs + D + 1), f, ls);
-      os = fmaf(__ldcg(w + (int64_t)k * cs + d), f, os);
-    }
-    put(rr, d, ls == 0.0f ? 0.0f : os / ls);
-  }
+  Place w = place;
+  at.run(w);
 }
 
-template <int NG>
-cudaError_t attn_launch(const Kv4AttnArgs& a, int64_t blocks, cudaStream_t st) {
-  constexpr int D = 32 * NG;
-  constexpr int smem = std::max(kAttnWarps * kStages * 20 * D, kAttnWarps * kRows * (D + 2) * 4);
-  // per device, and cheap: the attribute belongs to the current context
-  cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
+template <int NG, bool EXACT>
+cudaError_t attn_launch(Kv4AttnArgs a, int sm_count, cudaStream_t st) {
+  constexpr int smem = Attn<NG, EXACT>::kSmem;
+  static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(configured.load(std::memory_order_relaxed) & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<NG, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(bit, std::memory_order_relaxed);
+  }
+  // never more CTAs than the bounds on the lengths can give work to
+  const int64_t tiles = ((int64_t)a.max_q * (a.n_head / a.n_kv) + kRows - 1) / kRows;
+  const double most = (double)a.S * a.n_kv * tiles * (kUnitCost + (a.max_ctx + kTok - 1) / kTok);
+  const double want = most / a.min_share + 1.0;
+  const unsigned grid = (unsigned)std::min<double>(want, (double)std::min(kMaxCtas, kCtasPerSm * sm_count));
   count_launch();
-  kv4_attn_kernel<NG><<<(unsigned)blocks, kAttnThreads, smem, st>>>(a);
+  kv4_attn_kernel<NG, EXACT><<<grid, kAttnThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -879,36 +1191,22 @@ cudaError_t launch_kv4_read(const int* slots, int64_t n, int n_kv, int head_dim,
   return cudaGetLastError();
 }
 
-cudaError_t launch_kv4_attention(const Kv4Attention& c, int* plan_error) {
-  *plan_error = 0;
-  const int G = c.n_head / c.n_kv;
-  const int64_t tiles = ((int64_t)c.max_q * G + kRows - 1) / kRows;
-  const int64_t units = (int64_t)c.S * c.n_kv * tiles;
-  // Chunks: enough CTAs for two per SM when (sequence, head, tile) alone are fewer, and at
-  // most 2048 keys where lengths differ; none below 256 keys (four pages a warp).
-  int64_t chunk = 2048;
-  const int64_t want = (2 * (int64_t)c.sm_count + units - 1) / units;
-  if (want > 1) chunk = std::min<int64_t>(chunk, ((c.max_ctx + want - 1) / want + 63) / 64 * 64);
-  chunk = std::max<int64_t>(chunk, 256);
-  if ((c.max_ctx + chunk - 1) / chunk > 64) chunk = ((c.max_ctx + 63) / 64 + 63) / 64 * 64;
-  const int64_t slot = (int64_t)kRows * (c.head_dim + 2) * 4;
-  while (chunk < c.max_ctx && (units > c.count_words || units * ((c.max_ctx + chunk - 1) / chunk) * slot > (int64_t)c.ws_bytes))
-    chunk = units > c.count_words ? (c.max_ctx + 63) / 64 * 64 : 2 * chunk;
-  const int64_t chunks = (c.max_ctx + chunk - 1) / chunk;
-  const int64_t blocks = units * chunks;
-  if (blocks > INT32_MAX) {
-    *plan_error = 1;
-    return cudaSuccess;
-  }
-  Kv4AttnArgs a{c.q, c.q_dtype, c.ldq, (int)c.T, c.n_head, c.n_kv, c.scale, c.q_start, c.ctx_len, c.S, c.block_table,
-                c.max_blocks, c.max_q, c.max_ctx, c.pages, c.num_blocks, c.o, c.o_dtype, c.ldo, (int)tiles, (int)chunk,
-                (int)chunks, c.ws, c.count, c.status};
+cudaError_t launch_kv4_attention(const Kv4Attention& c) {
+  const int wide = c.q_dtype == 0 && c.ldq % 4 == 0 && reinterpret_cast<uintptr_t>(c.q) % 16 == 0;
+  const int wide_o = c.o_dtype == 0 && c.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(c.o) % 16 == 0;
+  Kv4AttnArgs a{c.q, c.q_dtype, wide, c.ldq, (int)c.T, c.n_head, c.n_kv, c.scale, c.q_start, c.ctx_len, c.S, c.block_table,
+                c.max_blocks, c.max_q, c.max_ctx, c.pages, c.num_blocks, c.o, c.o_dtype, wide_o,
+                c.ldo,                kUnitCost + std::min(32, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
+  const bool exact = c.o_dtype == 0;
   switch (c.head_dim / 32) {
-    case 1: return attn_launch<1>(a, blocks, c.stream);
-    case 2: return attn_launch<2>(a, blocks, c.stream);
-    case 3: return attn_launch<3>(a, blocks, c.stream);
-    default: return attn_launch<4>(a, blocks, c.stream);
+    case 1: return exact ? attn_launch<1, true>(a, c.sm_count, c.stream) : attn_launch<1, false>(a, c.sm_count, c.stream);
+    case 2: return exact ? attn_launch<2, true>(a, c.sm_count, c.stream) : attn_launch<2, false>(a, c.sm_count, c.stream);
+    case 3: return exact ? attn_launch<3, true>(a, c.sm_count, c.stream) : attn_launch<3, false>(a, c.sm_count, c.stream);
+    default: return exact ? attn_launch<4, true>(a, c.sm_count, c.stream) : attn_launch<4, false>(a, c.sm_count, c.stream);
   }
 }
+
+size_t kv4_attention_ws_bytes(int sm_count) { return (size_t)kCtasPerSm * sm_count * 2 * kRows * (128 + 2) * sizeof(float); }
+size_t kv4_attention_count_bytes(int sm_count) { return (size_t)kCtasPerSm * sm_count * sizeof(unsigned); }
 
 }  // namespace rtd
