@@ -10,16 +10,23 @@
 // cannot change a result, and every CTA of the cluster decides alike from the same
 // totals.  2^44 leaves room for 2^19 entries and drops what is below 2^-45 of the largest.
 //
-// A select finds the threshold where a count (top-k) or a weight (top-p) is reached:
-// first a histogram over 1024 equal steps of (max - x) / t, which spreads any row's upper
-// end over many bins; then, if at most 1023 entries share the bin, they are gathered and
-// ranked against one another, else the bin is split by the bits of the value's order map.
+// A histogram over 1024 equal steps of (max - x) / t spreads any row's upper end over many
+// bins.  With top-k, the bins that hold the k largest usually hold few more: they are
+// gathered into one CTA, which ranks them against one another and decides alone.  Where
+// they are too many, and for a nucleus over the whole row, a select finds the exact
+// threshold: the bin where the count or weight is reached, then, if at most 512 entries
+// share it, their ranks, else splits of it by the bits of the value's order map.
+//
+// Bound: for few rows the latency of the passes (three to five, the first from memory, the
+// others from L1) and of a cluster barrier after each; for many rows the 64-bit
+// exponentials of a nucleus over the whole row, else the passes' instructions.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "rtd_common.cuh"
@@ -30,17 +37,22 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024;
-constexpr int kBins = 1024;
-constexpr int kList = 1023;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 1024;  // two a thread
+constexpr int kList = 255;   // entries of a bin that are ranked against one another
+constexpr int kLanes = 4;    // threads that share an entry's comparisons
+constexpr int kCand = 1024;  // candidates that one CTA ranks, two a thread
 constexpr int kMaxRanks = 8;
+constexpr int kResident = 296;  // CTAs: more rows than fill the SMs get fewer CTAs each
 constexpr double kUnit = 17592186044416.0;  // 2^44
 
 struct SampleArgs {
   const void* x;
   int64_t ldx;
   int V;
-  int per_warp;  // entries of a warp, a multiple of 32
+  int per_warp;  // entries of a warp, a multiple of 256
+  int wide;      // rows on 16-byte boundaries
   const float* temperature;
   const int* top_k;
   const float* top_p;
@@ -68,42 +80,136 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 
 struct Shared {
   uint32_t cnt[2][kBins], lo[2][kBins], hi[2][kBins];
+  // candidates of the row (in rank 0), or a bin's entries
+  uint32_t keys[kCand], idx[kCand];
+  uint64_t weights[kCand];
+  uint32_t place[kCand];
   uint32_t list[kList + 1];
-  uint32_t keys[kList + 1];
-  uint64_t weights[kList + 1];
   uint64_t red[32];
   uint64_t red2[32];
-  uint64_t xch[4][2];  // values for the other CTAs, a slot per exchange
-  uint32_t list_n;
+  uint64_t xch[3][2];  // values for the other CTAs, a slot per exchange
+  uint32_t cand_n, list_n;
   uint32_t found, found_cnt;
-  uint64_t found_above;
+  uint64_t found_above, found_total;
+  double pow2[64];            // 2^(44 - i / 64)
+  float queue[kWarps][64];    // kept values waiting for a full warp of exponentials
 };
 
 template <int DT>
 struct Row {
+  static constexpr int kVec = DT == 0 ? 4 : 8;  // entries of 16 bytes
+  static constexpr int kAhead = DT == 0 ? 4 : 2;
   const SampleArgs& a;
   Shared& sm;
   cg::cluster_group cluster;
   const void* x;
   int rank, ranks, tid, lane, warp, w0, w1;
   float top, c;      // the row's maximum; histogram steps per unit of (max - x)
-  double inv_t, topd;
+  double topd, scale;  // log2(e) / t
   uint32_t sk;       // kept: keys above sk ...
   uint64_t sm_ties;  // ... and the first sm_ties entries with key sk
-  int buf = 0;
+  int buf;
 
+  // The weight of a value, rint(2^44 2^-y) with y = (max - v) log2(e) / t, in 64 bits:
+  // 2^(44 - i / 64) e^(-r ln 2) with i / 64 the 64th nearest y, the first from a table, the
+  // second by its Taylor series for |r| <= 2^-7, whose sixth term is below 2^-54.  40 cycles a
+  // warp, against 56 with exp().  From y = 46 on (-inf and NaN too) it is 0, without a branch.
   __device__ uint64_t weight(float v) const {
-    if (v == -INFINITY) return 0;
-    return (uint64_t)__double2ll_rn(exp(((double)v - topd) * inv_t) * kUnit);
+    const double y = fmin((topd - (double)v) * scale, 47.0);
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52
+    const double at = fma(y, 64.0, magic);
+    const int i = __double2loint(at);
+    const double r = fma(at - magic, -0.015625, y) * -0.69314718055994530942;
+    double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    e = fma(r, e, 1.0 / 6.0);
+    e = fma(r, e, 0.5);
+    e = fma(r, e, 1.0);
+    e = fma(r, e, 1.0);
+    const double f = sm.pow2[i & 63];
+    const double w = fma(__hiloint2double(__double2hiint(f) - ((i >> 6) << 20), __double2loint(f)), e, 4503599627370496.0);
+    return (uint64_t)__double_as_longlong(w) & 0xFFFFFFFFFFFFFull;  // rounded, in the mantissa under 2^52
+  }
+  // miss(value) for every entry, then f(value, weight) for those above `low`: where that is
+  // not all, few lanes of a warp hold one, and they wait for a full warp of exponentials.
+  template <typename F, typename G>
+  __device__ void weigh(float low, G miss, F f) {
+    if (low == -INFINITY) {
+      each<1>([&](int, float v) { f(v, weight(v)); });
+      return;
+    }
+    float* q = sm.queue[warp];
+    int waiting = 0;
+    each<1>([&](int, float v) {
+      miss(v);
+      const bool in = v > low;
+      const uint32_t late = __ballot_sync(0xffffffffu, in);
+      if (!late) return;
+      if (in) q[waiting + __popc(late & ((1u << lane) - 1u))] = v;
+      waiting += __popc(late);
+      __syncwarp();
+      if (waiting >= 32) {
+        const float x = q[lane];
+        f(x, weight(x));
+        waiting -= 32;
+        const float next = lane < waiting ? q[32 + lane] : 0.0f;
+        __syncwarp();
+        if (lane < waiting) q[lane] = next;
+        __syncwarp();
+      }
+    });
+    if (lane < waiting) f(q[lane], weight(q[lane]));
+    __syncwarp();
   }
   __device__ int bin(float v) const {
     const float t = (top - v) * c;
     return t < (float)(kBins - 1) ? (int)t : kBins - 1;
   }
-  template <typename F>
+  // kVec values from index i on; NaN past this warp's entries.
+  __device__ void vector_at(int i, float (&v)[kVec]) const {
+    if (i + kVec <= w1) {
+      if constexpr (DT == 0) {
+        const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
+        v[0] = q.x;
+        v[1] = q.y;
+        v[2] = q.z;
+        v[3] = q.w;
+      } else {
+        const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float2 y;
+          if constexpr (DT == 1)
+            y = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+          else
+            y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
+          v[2 * e] = y.x;
+          v[2 * e + 1] = y.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[e] = i + e < w1 ? load<DT>(x, i + e) : NAN;
+    }
+  }
+  // f(index, value) over this warp's entries, the whole warp in every call: lanes without
+  // an entry bring NaN.  AHEAD loads are in flight before the first use.
+  template <int AHEAD, typename F>
   __device__ void each(F f) const {
-#pragma unroll 4
-    for (int i = w0 + lane; i < w1; i += 32) f(i, load<DT>(x, i));
+    if (a.wide) {
+#pragma unroll 1
+      for (int i = w0 + lane * kVec; i - lane * kVec < w1; i += AHEAD * 32 * kVec) {
+        float v[AHEAD][kVec];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) vector_at(i + k * 32 * kVec, v[k]);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) f(i + k * 32 * kVec + e, v[k][e]);
+      }
+    } else {
+      for (int i = w0 + lane; i - lane < w1; i += 32) f(i, i < w1 ? load<DT>(x, i) : NAN);
+    }
   }
 
   __device__ uint64_t block_sum(uint64_t v, uint64_t* red) {
@@ -111,7 +217,7 @@ struct Row {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lane == 0) red[warp] = v;
     __syncthreads();
-    v = red[lane];
+    v = lane < kWarps ? red[lane] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     __syncthreads();
@@ -119,21 +225,31 @@ struct Row {
   }
 
   // Merge the cluster's histograms (buffer `buf`, already synchronised) and find the bin
-  // where `need` (>= 1) is reached; `tie_bin` holds `tie_n` more entries of weight `tie_w`.
-  template <bool W>
-  __device__ void find(uint64_t need, int tie_bin, uint64_t tie_n, uint64_t tie_w) {
-    uint64_t n = 0, v = 0;
+  // where need(total) >= 1 is reached, counts or weights; `tie_bin` holds `tie_n` more
+  // entries of weight `tie_w`.  Thread t has the bins 2 t and 2 t + 1.
+  template <bool W, typename F>
+  __device__ void find(F need_of, int tie_bin, uint64_t tie_n, uint64_t tie_w) {
+    uint64_t n[2] = {0, 0}, v[2] = {0, 0};
     for (int r = 0; r < ranks; ++r) {
       const Shared* o = cluster.map_shared_rank(&sm, r);
-      n += o->cnt[buf][tid];
-      if (W) v += (uint64_t)o->lo[buf][tid] + ((uint64_t)o->hi[buf][tid] << 32);
+      const uint2 q = reinterpret_cast<const uint2*>(o->cnt[buf])[tid];
+      n[0] += q.x;
+      n[1] += q.y;
+      if (W) {
+        const uint2 l = reinterpret_cast<const uint2*>(o->lo[buf])[tid], h = reinterpret_cast<const uint2*>(o->hi[buf])[tid];
+        v[0] += (uint64_t)l.x + ((uint64_t)h.x << 32);
+        v[1] += (uint64_t)l.y + ((uint64_t)h.y << 32);
+      }
     }
-    if (tid == tie_bin) {
-      n += tie_n;
-      v += tie_n * tie_w;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (2 * tid + e == tie_bin) {
+        n[e] += tie_n;
+        v[e] += tie_n * tie_w;
+      }
+      if (!W) v[e] = n[e];
     }
-    if (!W) v = n;
-    uint64_t inc = v;
+    uint64_t inc = v[0] + v[1];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
@@ -141,22 +257,30 @@ struct Row {
     }
     if (lane == 31) sm.red[warp] = inc;
     __syncthreads();
-    uint64_t before = lane < warp ? sm.red[lane] : 0;
+    uint64_t before = lane < warp ? sm.red[lane] : 0, total = lane < kWarps ? sm.red[lane] : 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
     inc += before;
-    if (inc >= need && inc - v < need) {
-      sm.found = (uint32_t)tid;
-      sm.found_cnt = (uint32_t)n;
-      sm.found_above = inc - v;
+    if (tid == 0) sm.found_total = total;
+    const uint64_t need = need_of(total);
+    uint64_t at = inc - v[0] - v[1];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (at < need && at + v[e] >= need) {
+        sm.found = (uint32_t)(2 * tid + e);
+        sm.found_cnt = (uint32_t)n[e];
+        sm.found_above = at;
+      }
+      at += v[e];
     }
     __syncthreads();
   }
 
   __device__ void clear_hist(int b) {
-    sm.cnt[b][tid] = 0;
-    sm.lo[b][tid] = 0;
-    sm.hi[b][tid] = 0;
+    for (int i = tid; i < kBins; i += kThreads) sm.cnt[b][i] = sm.lo[b][i] = sm.hi[b][i] = 0;
   }
 
   template <bool W>
@@ -170,22 +294,17 @@ struct Row {
   }
 
   // The kept set becomes its first entries, by value and then by index, that reach
-  // `target` (a count, or a weight when W); entries lighter than `floor_w` cannot be among
-  // them.  All CTAs of the cluster call it together.
-  template <bool W>
-  __device__ void select(uint64_t target, uint64_t floor_w) {
+  // need_of(the kept set's count or, when W, weight).  All CTAs of the cluster call it
+  // together.
+  template <bool W, typename F>
+  __device__ void select(F need_of) {
     const uint32_t sk0 = sk;
     const uint64_t ties = sm_ties;
-    const float tie_x = value_of(sk0);
+    const float tie_x = value_of(sk0), tie_v = sk0 ? tie_x : -INFINITY;  // a weight of -inf is 0
     const uint64_t tie_w = (W && ties) ? weight(tie_x) : 0;
-    // a value below which no weight reaches floor_w, with room for the roundings
-    float floor_x = -INFINITY;
-    if (W && floor_w > 1)
-      floor_x = top + (logf((float)floor_w * 5.6843418860808015e-14f) - 1e-3f) / (float)inv_t - 1e-6f * fabsf(top);
-    if (!(floor_x < top)) floor_x = -INFINITY;
-    uint64_t above = 0;
+    uint64_t above = 0, target = 0;
     int level = 0, b0 = 0;
-    uint32_t prefix = 0, n = 0;
+    uint32_t prefix = 0;
     const int shifts[5] = {0, 22, 12, 2, 0};
     auto digit = [&](uint32_t k, int lv) -> int {  // larger keys first
       return lv == 4 ? 3 - (int)(k & 3u) : 1023 - (int)((k >> shifts[lv]) & 1023u);
@@ -197,24 +316,22 @@ struct Row {
       return (k >> shifts[lv - 1]) == prefix;
     };
     for (;;) {
-      each([&](int, float v) {
+      each<1>([&](int, float v) {
+        if (!(v > tie_v)) return;  // NaN too
         const uint32_t k = key_of(v);
-        if (k <= sk0 || v < floor_x || !matches(v, k, level)) return;
-        uint64_t w = 0;
-        if (W) {
-          w = weight(v);
-          if (w < floor_w) return;
-        }
-        count_in<W>(level == 0 ? bin(v) : digit(k, level), w);
+        if (!matches(v, k, level)) return;
+        count_in<W>(level == 0 ? bin(v) : digit(k, level), W ? weight(v) : 0);
       });
       cluster.sync();
       const bool tie_in = W && ties && matches(tie_x, sk0, level);
-      find<W>(target - above, tie_in ? (level == 0 ? bin(tie_x) : digit(sk0, level)) : -1, ties, tie_w);
-      const int f = (int)sm.found;
-      n = sm.found_cnt;
-      above += sm.found_above;
+      find<W>([&](uint64_t total) { return level == 0 ? need_of(total) : target - above; },
+              tie_in ? (level == 0 ? bin(tie_x) : digit(sk0, level)) : -1, ties, tie_w);
       clear_hist(buf ^ 1);  // the other buffer was last read before this step's barrier
       buf ^= 1;
+      if (level == 0) target = need_of(sm.found_total);
+      const int f = (int)sm.found;
+      const uint32_t n = sm.found_cnt;
+      above += sm.found_above;
       if (level == 0)
         b0 = f;
       else if (level == 4)
@@ -233,42 +350,59 @@ struct Row {
     // gather the bin's entries and rank them
     if (tid == 0) sm.list_n = 0;
     __syncthreads();
-    each([&](int, float v) {
+    each<1>([&](int, float v) {
+      if (!(v > tie_v) || bin(v) != b0) return;
       const uint32_t k = key_of(v);
-      if (k <= sk0 || v < floor_x || !matches(v, k, level)) return;
-      if (W && floor_w > 1 && weight(v) < floor_w) return;
+      if (!matches(v, k, level)) return;
       const uint32_t at = atomicAdd(&sm.list_n, 1u);
       if (at < (uint32_t)kList) sm.list[at] = k;
     });
     cluster.sync();
+    settle<W>(above, target, W && ties && matches(tie_x, sk0, level), sk0, ties);
+  }
+
+  // Ranks the entries that the CTAs' lists hold (already synchronised), at most kList in
+  // all, and `ties` more of key tie_key where tie_in: the threshold where `target` is
+  // reached, `above` lying before them.
+  template <bool W>
+  __device__ void settle(uint64_t above, uint64_t target, bool tie_in, uint32_t tie_key, uint64_t ties) {
     uint32_t total = 0;
     for (int r = 0; r < ranks; ++r) {
       const Shared* o = cluster.map_shared_rank(&sm, r);
       const uint32_t m = min(o->list_n, (uint32_t)kList);
-      if (tid < (int)m && total + tid <= (uint32_t)kList) sm.keys[total + tid] = o->list[tid];
+      for (uint32_t i = tid; i < m && total + i < (uint32_t)kCand; i += kThreads) sm.keys[total + i] = o->list[i];
       total += m;
     }
-    const bool tie_in = W && ties && matches(tie_x, sk0, level);
-    if (tie_in && tid == 0 && total <= (uint32_t)kList) sm.keys[total] = sk0;
+    if (tie_in && tid == 0 && total < (uint32_t)kCand) sm.keys[total] = tie_key;
     if (tie_in) ++total;
-    total = min(total, (uint32_t)kList + 1u);
+    total = min(total, (uint32_t)kCand);
     __syncthreads();
-    const bool mine = tid < (int)total;
-    const uint32_t k = mine ? sm.keys[tid] : 0;
-    const uint64_t w1 = mine ? (W ? weight(value_of(k)) : 1) : 0;
-    if (mine) sm.weights[tid] = (tie_in && tid == (int)total - 1) ? ties * w1 : w1;
+    for (uint32_t i = tid; i < total; i += kThreads) {
+      const uint64_t w = W ? weight(value_of(sm.keys[i])) : 1;
+      sm.weights[i] = (tie_in && i == total - 1) ? ties * w : w;
+    }
     __syncthreads();
-    if (mine) {
-      uint64_t gt = above, eq = 0;
-      for (uint32_t j = 0; j < total; ++j) {
+    for (uint32_t i0 = 0; i0 < total; i0 += kThreads / kLanes) {
+      const uint32_t i = i0 + tid / kLanes;
+      const uint32_t k = i < total ? sm.keys[i] : 0;
+      uint64_t gt = 0, eq = 0;
+#pragma unroll 4
+      for (uint32_t j = tid % kLanes; j < total; j += kLanes) {
         const uint32_t kj = sm.keys[j];
         const uint64_t wj = sm.weights[j];
-        if (kj > k) gt += wj;
-        if (kj == k) eq += wj;
+        gt += kj > k ? wj : 0;
+        eq += kj == k ? wj : 0;
       }
-      if (gt < target && gt + eq >= target) {
+#pragma unroll
+      for (int o = 1; o < kLanes; o *= 2) {
+        gt += __shfl_xor_sync(0xffffffffu, gt, o);
+        eq += __shfl_xor_sync(0xffffffffu, eq, o);
+      }
+      gt += above;
+      if (i < total && gt < target && gt + eq >= target) {
+        const uint64_t w = W ? weight(value_of(k)) : 1;
         sm.found = k;
-        sm.found_above = (target - gt + w1 - 1) / w1;
+        sm.found_above = (target - gt + w - 1) / w;
       }
     }
     __syncthreads();
@@ -277,78 +411,300 @@ struct Row {
     __syncthreads();
   }
 
-  __device__ void run(int row) {
-    // ---- the largest value and its lowest index
-    uint64_t best = 0, valid = 0;
-    each([&](int i, float v) {
-      const uint32_t k = key_of(v);
-      valid += k != 0;
-      const uint64_t p = ((uint64_t)k << 32) | (uint32_t)(0xffffffffu - (uint32_t)i);
-      if (k && p > best) best = p;
+  // The nucleus of the whole row.  A histogram of counts and of places within the bins
+  // brackets each bin's weight: with f the mean place, n e^(-step f) is a lower bound (the
+  // exponential is convex) and 1 + step^2 / 8 < 1.0003 times that an upper one.  The exact
+  // pass then sums what lies before the bins that may hold the threshold, and the whole,
+  // and gathers those bins' entries, or, where they are too many, a finer histogram of them.
+  // False: too many even so.
+  __device__ bool nucleus_of_row(float p) {
+    constexpr double kStep = 31.9 / kBins;
+    each<kAhead>([&](int, float v) {
+      const float t = (top - v) * c;
+      if (!(t < (float)kBins)) return;  // NaN, and what weighs nothing
+      const int b = (int)t;
+      atomicAdd(&sm.cnt[buf][b], 1u);
+      atomicAdd(&sm.lo[buf][b], (uint32_t)((t - (float)b) * 4096.0f));
     });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) sm.red2[warp] = best;
-    clear_hist(0);
-    clear_hist(1);
-    valid = block_sum(valid, sm.red);
-    best = sm.red2[lane];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (tid == 0) {
-      sm.xch[0][0] = best;
-      sm.xch[0][1] = valid;
-    }
+    if (tid == 0) sm.list_n = 0;
     cluster.sync();
-    valid = 0;
+    uint64_t n[2] = {0, 0}, f[2] = {0, 0};
     for (int r = 0; r < ranks; ++r) {
       const Shared* o = cluster.map_shared_rank(&sm, r);
-      best = max(best, o->xch[0][0]);
-      valid += o->xch[0][1];
+      const uint2 q = reinterpret_cast<const uint2*>(o->cnt[buf])[tid], g = reinterpret_cast<const uint2*>(o->lo[buf])[tid];
+      n[0] += q.x;
+      n[1] += q.y;
+      f[0] += g.x;
+      f[1] += g.y;
     }
-    top = value_of((uint32_t)(best >> 32));
+    // the lower bounds in units of 2^-40 of the largest weight: whole numbers again, so that
+    // every CTA finds the same bins
+    uint64_t w[2], inc[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      w[e] = n[e] ? (uint64_t)((double)n[e] * exp(-kStep * ((double)(2 * tid + e) + (double)f[e] / (4096.0 * (double)n[e]))) *
+                               1099511627776.0)
+                  : 0;
+      inc[0] += w[e];
+      inc[1] += n[e];
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, inc[e], o);
+        if (lane >= o) inc[e] += y;
+      }
+    if (lane == 31) {
+      sm.red[warp] = inc[0];
+      sm.red2[warp] = inc[1];
+    }
+    __syncthreads();
+    uint64_t all = 0;
+    for (int k = 0; k < kWarps; ++k) {
+      if (k < warp) {
+        inc[0] += sm.red[k];
+        inc[1] += sm.red2[k];
+      }
+      all += sm.red[k];
+    }
+    const double part = (double)p * (double)all;
+    const uint64_t low = max((uint64_t)1, (uint64_t)(part * 0.9996)), high = max(low, min(all, (uint64_t)(part * 1.0004) + 1));
+    uint64_t at = inc[0] - w[0] - w[1], many = inc[1] - n[0] - n[1];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (at < low && at + w[e] >= low) {
+        sm.found = (uint32_t)(2 * tid + e);
+        sm.found_above = many;
+      }
+      if (at < high && at + w[e] >= high) {
+        sm.found_cnt = (uint32_t)(2 * tid + e);
+        sm.found_total = many + n[e];
+      }
+      at += w[e];
+      many += n[e];
+    }
+    __syncthreads();
+    const float from = (float)sm.found, upto = (float)(sm.found_cnt + 1);
+    const bool few = sm.found_total - sm.found_above <= (uint64_t)kList;
+    buf ^= 1;
+    const float fine = (float)kBins / (upto - from);
+    auto fine_bin = [&](float t) { return min((int)((t - from) * fine), kBins - 1); };
+    uint64_t z = 0, before = 0;
+    weigh(-INFINITY, [](float) {}, [&](float v, uint64_t e) {
+      const float t = (top - v) * c;
+      z += e;
+      before += t < from ? e : 0;
+      if (t >= from && t < upto) {
+        if (few) {
+          const uint32_t at = atomicAdd(&sm.list_n, 1u);
+          if (at < (uint32_t)kList) sm.list[at] = key_of(v);
+        } else {
+          count_in<true>(fine_bin(t), e);
+        }
+      }
+    });
+    z = block_sum(z, sm.red);
+    before = block_sum(before, sm.red);
+    if (tid == 0) {
+      sm.xch[2][0] = z;
+      sm.xch[2][1] = before;
+    }
+    cluster.sync();
+    z = before = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const Shared* o = cluster.map_shared_rank(&sm, r);
+      z += o->xch[2][0];
+      before += o->xch[2][1];
+    }
+    const uint64_t target = nucleus(p, z);
+    if (!few) {
+      find<true>([&](uint64_t) { return target - before; }, -1, 0, 0);
+      const int fb = (int)sm.found;
+      before += sm.found_above;
+      const bool fits = sm.found_cnt <= (uint32_t)kList;
+      clear_hist(buf ^ 1);
+      buf ^= 1;
+      __syncthreads();
+      if (!fits) return false;
+      each<kAhead>([&](int, float v) {
+        const float t = (top - v) * c;
+        if (!(t >= from && t < upto) || fine_bin(t) != fb) return;
+        const uint32_t at = atomicAdd(&sm.list_n, 1u);
+        if (at < (uint32_t)kList) sm.list[at] = key_of(v);
+      });
+      cluster.sync();
+    }
+    settle<true>(before, target, false, 0, 0);
+    return true;
+  }
+
+  // floor(u * total), within 0 .. total - 1
+  __device__ static uint64_t drawn(float u, uint64_t total) {
+    const double e = floor((double)(u > 0.0f ? u : 0.0f) * (double)total);
+    return e < (double)total ? min((uint64_t)e, total - 1) : total - 1;
+  }
+  __device__ static uint64_t nucleus(float p, uint64_t total) {
+    const double e = floor((double)p * (double)total);
+    return e >= 1.0 ? min(total, (uint64_t)e) : 1;
+  }
+
+  // The k largest are among n <= kCand candidates: rank 0 decides on them alone.
+  __device__ void among(int n, int k, float p, uint64_t least, float u, int row) {
+    const int most = min(n, k);
+    // ranks, and the weights in order of rank
+    for (int i0 = 0; i0 < n; i0 += kThreads / kLanes) {
+      const int i = i0 + tid / kLanes;
+      const uint32_t key = i < n ? sm.keys[i] : 0, id = i < n ? sm.idx[i] : 0;
+      uint32_t place = 0;
+#pragma unroll 4
+      for (int j = tid % kLanes; j < n; j += kLanes) {
+        const uint32_t kj = sm.keys[j];
+        place += kj > key || (kj == key && sm.idx[j] < id);
+      }
+#pragma unroll
+      for (int o = 1; o < kLanes; o *= 2) place += __shfl_xor_sync(0xffffffffu, place, o);
+      if (i < n && tid % kLanes == 0) {
+        sm.place[i] = place;
+        sm.weights[place] = place < (uint32_t)most ? weight(value_of(key)) : 0;
+      }
+    }
+    __syncthreads();
+    uint64_t w[2] = {2 * tid < most ? sm.weights[2 * tid] : 0, 2 * tid + 1 < most ? sm.weights[2 * tid + 1] : 0};
+    if (p < 1.0f) {  // in order of rank, those before which `enough` is not reached yet
+      uint64_t inc = w[0] + w[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      if (lane == 31) sm.red[warp] = inc;
+      __syncthreads();
+      uint64_t before = inc - w[0] - w[1], total = 0;
+      for (int e = 0; e < kWarps; ++e) {
+        if (e < warp) before += sm.red[e];
+        total += sm.red[e];
+      }
+      const uint64_t enough = nucleus(p, total);
+      if (before + w[0] >= enough) w[1] = 0;
+      if (before >= enough) w[0] = 0;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (w[e] < least) w[e] = 0;
+      if (2 * tid + e < n) sm.weights[2 * tid + e] = w[e];
+    }
+    const uint64_t at = drawn(u, block_sum(w[0] + w[1], sm.red));
+    // the pick, in index order
+    for (int i0 = 0; i0 < n; i0 += kThreads / kLanes) {
+      const int i = i0 + tid / kLanes;
+      const uint32_t id = i < n ? sm.idx[i] : 0;
+      uint64_t before = 0;
+#pragma unroll 4
+      for (int j = tid % kLanes; j < n; j += kLanes) before += sm.idx[j] < id ? sm.weights[sm.place[j]] : 0;
+#pragma unroll
+      for (int o = 1; o < kLanes; o *= 2) before += __shfl_xor_sync(0xffffffffu, before, o);
+      if (i < n && tid % kLanes == 0 && before <= at && at < before + sm.weights[sm.place[i]]) a.ids[row] = (int)id;
+    }
+  }
+
+  __device__ void run(int row) {
+    // ---- the largest value and its lowest index
     const float t = a.temperature ? a.temperature[row] : 1.0f;
     const int k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.0f;
+    const float mp = a.min_p ? a.min_p[row] : 0.0f;
+    const float u = a.u[row];
+    float mine = -INFINITY;
+    int mine_i = -1;
+    each<kAhead>([&](int i, float v) {
+      if (v > mine) {  // a lane meets its entries in index order
+        mine = v;
+        mine_i = i;
+      }
+    });
+    if (mine_i < 0) {  // nothing above -inf: its first -inf, if any
+      each<1>([&](int i, float v) {
+        if (v == -INFINITY && mine_i < 0) mine_i = i;
+      });
+    }
+    uint64_t best = mine_i >= 0 ? ((uint64_t)key_of(mine) << 32) | (0xffffffffu - (uint32_t)mine_i) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) sm.red[warp] = best;
+    if (tid == 0) sm.cand_n = 0;
+    if (tid < 64) sm.pow2[tid] = exp2(44.0 - (double)tid / 64.0);
+    buf = 0;
+    clear_hist(0);
+    clear_hist(1);
+    __syncthreads();
+    if (warp == 0) {
+      uint64_t b = lane < kWarps ? sm.red[lane] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+      if (lane == 0) sm.xch[0][0] = b;
+    }
+    cluster.sync();
+    best = 0;
+    for (int r = 0; r < ranks; ++r) best = max(best, cluster.map_shared_rank(&sm, r)->xch[0][0]);
+    top = value_of((uint32_t)(best >> 32));
     if (best == 0 || !(fabsf(top) < INFINITY) || !(t > 0.0f) || k == 1) {
       if (rank == 0 && tid == 0) a.ids[row] = best == 0 ? 0 : (int)(0xffffffffu - (uint32_t)best);
       return;
     }
     topd = (double)top;
-    inv_t = 1.0 / (double)t;
+    scale = 1.4426950408889634074 / (double)t;
     c = fminf((float)kBins / 31.9f / t, 1e30f);  // 46 ln 2: beyond it a weight is zero
     sk = 0;
     sm_ties = 0;
+    const uint64_t least = mp > 0.0f ? (uint64_t)ceil((double)fminf(mp, 1.0f) * kUnit) : 0;
     // ---- filters
-    if (k > 0 && (uint64_t)k < valid) select<false>((uint64_t)k, 0);
-    const float p = a.top_p ? a.top_p[row] : 1.0f;
-    if (p < 1.0f) {
-      uint64_t z = 0;
-      each([&](int, float v) {
-        if (key_of(v) > sk) z += weight(v);
-      });
-      z = block_sum(z, sm.red);
-      if (tid == 0) sm.xch[1][0] = z;
-      cluster.sync();
-      z = sm_ties ? sm_ties * weight(value_of(sk)) : 0;
-      for (int r = 0; r < ranks; ++r) z += cluster.map_shared_rank(&sm, r)->xch[1][0];
-      const double e = floor((double)p * (double)z);
-      const uint64_t target = e >= 1.0 ? min(z, (uint64_t)e) : 1;
-      select<true>(target, (z - target) / (uint64_t)a.V);
+    if (k > 0 && k < a.V) {
+      // The lanes' maxima bound the k-th largest from below: at least k entries lie in the
+      // bins up to the one where the maxima reach k, and with many more lanes than k few
+      // others do.
+      bool few = 2 * k <= ranks * kThreads;
+      if (few) {
+        if (mine > -INFINITY) atomicAdd(&sm.cnt[0][bin(mine)], 1u);
+        cluster.sync();
+        find<false>([&](uint64_t total) { return total >= (uint64_t)k ? (uint64_t)k : 0; }, -1, 0, 0);
+        few = sm.found_total >= (uint64_t)k && sm.found < (uint32_t)kBins - 1;
+        clear_hist(1);
+        buf = 1;
+      }
+      if (few) {
+        const float upto = (float)(sm.found + 1);
+        Shared* o = cluster.map_shared_rank(&sm, 0);
+        each<kAhead>([&](int i, float v) {
+          if (!((top - v) * c < upto)) return;
+          const uint32_t at = atomicAdd(&o->cand_n, 1u);
+          if (at < (uint32_t)kCand) {
+            o->keys[at] = key_of(v);
+            o->idx[at] = (uint32_t)i;
+          }
+        });
+        cluster.sync();
+        const uint32_t n = o->cand_n;
+        if (n <= (uint32_t)kCand) {
+          if (rank == 0) among((int)n, k, p, least, u, row);
+          return;
+        }
+      }
+      select<false>([&](uint64_t total) { return min((uint64_t)k, total); });
     }
-    const float mp = a.min_p ? a.min_p[row] : 0.0f;
-    const double least = mp > 0.0f ? (double)fminf(mp, 1.0f) * kUnit : 0.0;
+    if (p < 1.0f && (sk || !nucleus_of_row(p))) select<true>([&](uint64_t total) { return nucleus(p, total); });
     auto kept_weight = [&](float v) -> uint64_t {
       const uint64_t w = weight(v);
-      return (double)w >= least ? w : 0;
+      return w >= least ? w : 0;
     };
     // ---- the pick
     const uint64_t tie_w = sm_ties ? kept_weight(value_of(sk)) : 0;
-    uint64_t z = 0, ties = 0;
-    each([&](int, float v) {
-      const uint32_t key = key_of(v);
-      if (key > sk) z += kept_weight(v);
-      if (sm_ties && key == sk) ++ties;
-    });
+    const float kept_above = sk ? value_of(sk) : -INFINITY;  // a weight of -inf is 0
+    uint64_t z = 0;
+    uint32_t ties = 0;
+    weigh(kept_above, [&](float v) { ties += v == kept_above; }, [&](float, uint64_t w) { z += w >= least ? w : 0; });
+    if (!sm_ties) ties = 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       z += __shfl_xor_sync(0xffffffffu, z, o);
@@ -360,15 +716,15 @@ struct Row {
     }
     __syncthreads();
     if (warp == 0) {
-      uint64_t zz = sm.red[lane], tt = sm.red2[lane];
+      uint64_t zz = lane < kWarps ? sm.red[lane] : 0, tt = lane < kWarps ? sm.red2[lane] : 0;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         zz += __shfl_xor_sync(0xffffffffu, zz, o);
         tt += __shfl_xor_sync(0xffffffffu, tt, o);
       }
       if (lane == 0) {
-        sm.xch[2][0] = zz;
-        sm.xch[2][1] = tt;
+        sm.xch[1][0] = zz;
+        sm.xch[1][1] = tt;
       }
     }
     cluster.sync();
@@ -376,57 +732,85 @@ struct Row {
     for (int r = 0; r < ranks; ++r) {
       const Shared* o = cluster.map_shared_rank(&sm, r);
       if (r < rank) {
-        base += o->xch[2][0];
-        tie_base += o->xch[2][1];
+        base += o->xch[1][0];
+        tie_base += o->xch[1][1];
       }
-      total += o->xch[2][0];
+      total += o->xch[1][0];
     }
     total += sm_ties * tie_w;
-    const float u = a.u[row];
-    const double e = floor((double)(u > 0.0f ? u : 0.0f) * (double)total);
-    const uint64_t at = e < (double)total ? min((uint64_t)e, total - 1) : total - 1;
-    for (int w = 0; w < warp; ++w) {
-      base += sm.red[w];
-      tie_base += sm.red2[w];
-    }
+    const uint64_t at = drawn(u, total);
     // weight kept before an entry = what lies above sk + the ties kept so far
     auto ties_kept = [&](uint64_t n) { return min(n, sm_ties) * tie_w; };
-    const uint64_t from = base + ties_kept(tie_base);
-    const uint64_t to = base + sm.red[warp] + ties_kept(tie_base + sm.red2[warp]);
-    if (at < from || at >= to) return;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-      const int i = i0 + lane;
-      const float v = i < w1 ? load<DT>(x, i) : NAN;
-      const uint32_t key = key_of(v);
-      const bool tie = sm_ties && key == sk && i < w1;
-      uint64_t w = key > sk ? kept_weight(v) : 0;
-      const uint32_t tied = __ballot_sync(0xffffffffu, tie);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += y;
+    if (tid == 0) sm.found = kWarps;
+    __syncthreads();
+    if (lane == 0) {
+      for (int w = 0; w < warp; ++w) {
+        base += sm.red[w];
+        tie_base += sm.red2[w];
       }
-      const uint64_t reached = base + w + ties_kept(tie_base + __popc(tied & (0xffffffffu >> (31 - lane))));
-      const uint32_t past = __ballot_sync(0xffffffffu, reached > at);
-      if (past) {
-        if (lane == __ffs(past) - 1) a.ids[row] = i;
+      if (at >= base + ties_kept(tie_base) && at < base + sm.red[warp] + ties_kept(tie_base + sm.red2[warp])) {
+        sm.found = (uint32_t)warp;
+        sm.found_above = base;
+        sm.found_total = tie_base;
+      }
+    }
+    __syncthreads();
+    if (sm.found == kWarps) return;
+    // the CTA shares the entries of that warp, a stretch a thread, and scans them
+    base = sm.found_above;
+    tie_base = sm.found_total;
+    const int64_t start = (int64_t)(rank * kWarps + (int)sm.found) * a.per_warp;
+    const int per = a.per_warp / 256, stop = (int)min(start + a.per_warp, (int64_t)a.V);
+    const int i0 = (int)min(start + (int64_t)tid * per, (int64_t)stop), i1 = tid < 256 ? min(i0 + per, stop) : i0;
+    uint64_t w = 0, tied = 0;
+    for (int i = i0; i < i1; ++i) {
+      const float v = load<DT>(x, i);
+      if (v > kept_above) w += kept_weight(v);
+      tied += sm_ties && v == kept_above;
+    }
+    uint64_t w_in = w, t_in = tied;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, w_in, o), t = __shfl_up_sync(0xffffffffu, t_in, o);
+      if (lane >= o) {
+        w_in += y;
+        t_in += t;
+      }
+    }
+    __syncthreads();
+    if (lane == 31) {
+      sm.red[warp] = w_in;
+      sm.red2[warp] = t_in;
+    }
+    __syncthreads();
+    for (int k = 0; k < warp; ++k) {
+      base += sm.red[k];
+      tie_base += sm.red2[k];
+    }
+    base += w_in - w;
+    tie_base += t_in - tied;
+    if (at < base + ties_kept(tie_base) || at >= base + w + ties_kept(tie_base + tied)) return;
+    for (int i = i0; i < i1; ++i) {
+      const float v = load<DT>(x, i);
+      if (v > kept_above) base += kept_weight(v);
+      tie_base += sm_ties && v == kept_above;
+      if (base + ties_kept(tie_base) > at) {
+        a.ids[row] = i;
         return;
       }
-      base += __shfl_sync(0xffffffffu, w, 31);
-      tie_base += __popc(tied);
     }
   }
 };
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sm = *reinterpret_cast<Shared*>(smem);
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = (int)(blockIdx.x / ranks);
   const int tid = threadIdx.x, warp = tid >> 5;
-  const int64_t first = (int64_t)(rank * (kThreads / 32) + warp) * a.per_warp;
+  const int64_t first = (int64_t)(rank * kWarps + warp) * a.per_warp;
   constexpr int es = DT == 0 ? 4 : 2;
   Row<DT> r{a, sm, cluster, static_cast<const uint8_t*>(a.x) + (int64_t)row * a.ldx * es, rank, ranks, tid, tid & 31, warp,
             (int)min(first, (int64_t)a.V), (int)min(first + a.per_warp, (int64_t)a.V)};
@@ -434,16 +818,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
   cluster.sync();  // no CTA leaves while another may read its shared memory
 }
 
-}  // namespace
-
-cudaError_t launch_sample(const void* x, int dt, int64_t ldx, int64_t T, int64_t V, const float* temperature,
-                          const int* top_k, const float* top_p, const float* min_p, const float* u, int* ids,
-                          cudaStream_t st) {
-  if (T <= 0) return cudaSuccess;
-  int ranks = 1;
-  while (ranks < kMaxRanks && V > (int64_t)ranks * 8 * kThreads) ranks *= 2;
-  const int64_t warps = (int64_t)ranks * (kThreads / 32);
-  SampleArgs a{x, ldx, (int)V, (int)(((V + warps - 1) / warps + 31) / 32 * 32), temperature, top_k, top_p, min_p, u, ids};
+template <int DT>
+cudaError_t sample_launch(const SampleArgs& a, int64_t T, int ranks, cudaStream_t st) {
+  static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(configured.load(std::memory_order_relaxed) & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(bit, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(T * ranks));
   cfg.blockDim = dim3(kThreads);
@@ -456,10 +841,22 @@ cudaError_t launch_sample(const void* x, int dt, int64_t ldx, int64_t T, int64_t
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  auto go = [&](auto k) {
-    return cudaLaunchKernelEx(&cfg, k, a);
-  };
-  return dt == 0 ? go(sample_kernel<0>) : dt == 1 ? go(sample_kernel<1>) : go(sample_kernel<2>);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<DT>, a);
+}
+
+}  // namespace
+
+cudaError_t launch_sample(const void* x, int dt, int64_t ldx, int64_t T, int64_t V, const float* temperature,
+                          const int* top_k, const float* top_p, const float* min_p, const float* u, int* ids,
+                          cudaStream_t st) {
+  if (T <= 0) return cudaSuccess;
+  int ranks = 1;
+  while (ranks < kMaxRanks && V > (int64_t)ranks * 8 * kThreads && 2 * ranks * T <= kResident) ranks *= 2;
+  const int64_t warps = (int64_t)ranks * kWarps;
+  const int es = dt == 0 ? 4 : 2;
+  const int wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (T == 1 || ldx * es % 16 == 0);
+  SampleArgs a{x, ldx, (int)V, (int)(((V + warps - 1) / warps + 255) / 256 * 256), wide, temperature, top_k, top_p, min_p, u, ids};
+  return dt == 0 ? sample_launch<0>(a, T, ranks, st) : dt == 1 ? sample_launch<1>(a, T, ranks, st) : sample_launch<2>(a, T, ranks, st);
 }
 
 }  // namespace rtd
