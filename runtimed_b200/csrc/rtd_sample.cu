@@ -37,13 +37,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 1024;  // two a thread
+constexpr int kBins = 1024;
 constexpr int kList = 255;   // entries of a bin that are ranked against one another
 constexpr int kLanes = 4;    // threads that share an entry's comparisons
-constexpr int kCand = 1024;  // candidates that one CTA ranks, two a thread
+constexpr int kCand = 1024;  // candidates that one CTA ranks
 constexpr int kMaxRanks = 8;
+constexpr int kNT = 512;
 constexpr int kResident = 296;  // CTAs: more rows than fill the SMs get fewer CTAs each
 constexpr double kUnit = 17592186044416.0;  // 2^44
 
@@ -88,17 +87,20 @@ struct Shared {
   uint64_t red[32];
   uint64_t red2[32];
   uint64_t xch[3][2];  // values for the other CTAs, a slot per exchange
-  uint32_t cand_n, list_n;
+  uint32_t cand_n, list_n, first;
   uint32_t found, found_cnt;
   uint64_t found_above, found_total;
   double pow2[64];            // 2^(44 - i / 64)
-  float queue[kWarps][64];    // kept values waiting for a full warp of exponentials
+  float queue[32][64];        // kept values waiting for a full warp of exponentials
 };
 
-template <int DT>
+template <int DT, int NT>
 struct Row {
+  static constexpr int kWarps = NT / 32;
+  static constexpr int kPer = kBins / NT;       // bins, or candidates, of a thread
   static constexpr int kVec = DT == 0 ? 4 : 8;  // entries of 16 bytes
-  static constexpr int kAhead = DT == 0 ? 4 : 2;
+  static constexpr int kAhead = DT == 0 ? 4 : 2;  // loads in flight where every entry is looked at,
+  static constexpr int kFar = 4;                  // and where few are
   const SampleArgs& a;
   Shared& sm;
   cg::cluster_group cluster;
@@ -164,32 +166,55 @@ struct Row {
     const float t = (top - v) * c;
     return t < (float)(kBins - 1) ? (int)t : kBins - 1;
   }
-  // kVec values from index i on; NaN past this warp's entries.
-  __device__ void vector_at(int i, float (&v)[kVec]) const {
+  // The 16 bytes from index i on; NaN past this warp's entries.
+  __device__ uint4 raw_at(int i) const {
     if (i + kVec <= w1) {
-      if constexpr (DT == 0) {
-        const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
-        v[0] = q.x;
-        v[1] = q.y;
-        v[2] = q.z;
-        v[3] = q.w;
-      } else {
-        const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+      if constexpr (DT == 0)
+        return *reinterpret_cast<const uint4*>(static_cast<const float*>(x) + i);
+      else
+        return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i);
+    }
+    uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};  // NaN in every type
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float2 y;
-          if constexpr (DT == 1)
-            y = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-          else
-            y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
-          v[2 * e] = y.x;
-          v[2 * e + 1] = y.y;
-        }
+    for (int e = 0; e < kVec; ++e)
+      if (i + e < w1) {
+        if constexpr (DT == 0)
+          w[e] = static_cast<const uint32_t*>(x)[i + e];
+        else
+          w[e / 2] = (e & 1) ? (w[e / 2] & 0xffffu) | ((uint32_t) static_cast<const uint16_t*>(x)[i + e] << 16)
+                             : (w[e / 2] & 0xffff0000u) | static_cast<const uint16_t*>(x)[i + e];
       }
-    } else {
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ static void unpack(uint4 q, float (&v)[kVec]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[e] = i + e < w1 ? load<DT>(x, i + e) : NAN;
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (DT == 0) {
+        v[e] = __uint_as_float(w[e]);
+      } else {
+        float2 y;
+        if constexpr (DT == 1)
+          y = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+        else
+          y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
+        v[2 * e] = y.x;
+        v[2 * e + 1] = y.y;
+      }
+    }
+  }
+  // The largest of them that is no NaN.
+  __device__ static float largest(uint4 q) {
+    if constexpr (DT == 0) {
+      return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+    } else if constexpr (DT == 1) {
+      auto h = [](uint32_t u) { return *reinterpret_cast<__half2*>(&u); };
+      const float2 m = __half22float2(__hmax2(__hmax2(h(q.x), h(q.y)), __hmax2(h(q.z), h(q.w))));
+      return fmaxf(m.x, m.y);
+    } else {
+      auto h = [](uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); };
+      const float2 m = __bfloat1622float2(__hmax2(__hmax2(h(q.x), h(q.y)), __hmax2(h(q.z), h(q.w))));
+      return fmaxf(m.x, m.y);
     }
   }
   // f(index, value) over this warp's entries, the whole warp in every call: lanes without
@@ -199,16 +224,59 @@ struct Row {
     if (a.wide) {
 #pragma unroll 1
       for (int i = w0 + lane * kVec; i - lane * kVec < w1; i += AHEAD * 32 * kVec) {
-        float v[AHEAD][kVec];
+        uint4 q[AHEAD];
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) vector_at(i + k * 32 * kVec, v[k]);
+        for (int k = 0; k < AHEAD; ++k) q[k] = raw_at(i + k * 32 * kVec);
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
+        for (int k = 0; k < AHEAD; ++k) {
+          float v[kVec];
+          unpack(q[k], v);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) f(i + k * 32 * kVec + e, v[k][e]);
+          for (int e = 0; e < kVec; ++e) f(i + k * 32 * kVec + e, v[e]);
+        }
       }
     } else {
       for (int i = w0 + lane; i - lane < w1; i += 32) f(i, i < w1 ? load<DT>(x, i) : NAN);
+    }
+  }
+
+  // f(largest of a few entries), covering this warp's; NaN counts for nothing.
+  template <typename F>
+  __device__ void each_max(F f) const {
+    if (a.wide) {
+#pragma unroll 1
+      for (int i = w0 + lane * kVec; i - lane * kVec < w1; i += kFar * 32 * kVec) {
+        uint4 q[kFar];
+#pragma unroll
+        for (int k = 0; k < kFar; ++k) q[k] = raw_at(i + k * 32 * kVec);
+#pragma unroll
+        for (int k = 0; k < kFar; ++k) f(largest(q[k]));
+      }
+    } else {
+      for (int i = w0 + lane; i < w1; i += 32) f(load<DT>(x, i));
+    }
+  }
+  // f(index, value) at least for the entries that are not below `low` (few of them).
+  template <typename F>
+  __device__ void each_from(float low, F f) const {
+    if (a.wide) {
+#pragma unroll 1
+      for (int i = w0 + lane * kVec; i - lane * kVec < w1; i += kFar * 32 * kVec) {
+        uint4 q[kFar];
+#pragma unroll
+        for (int k = 0; k < kFar; ++k) q[k] = raw_at(i + k * 32 * kVec);
+#pragma unroll
+        for (int k = 0; k < kFar; ++k)
+          if (largest(q[k]) >= low) {
+            float v[kVec];
+            unpack(q[k], v);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e)
+              if (v[e] >= low) f(i + k * 32 * kVec + e, v[e]);
+          }
+      }
+    } else {
+      for (int i = w0 + lane; i < w1; i += 32) f(i, load<DT>(x, i));
     }
   }
 
@@ -226,30 +294,36 @@ struct Row {
 
   // Merge the cluster's histograms (buffer `buf`, already synchronised) and find the bin
   // where need(total) >= 1 is reached, counts or weights; `tie_bin` holds `tie_n` more
-  // entries of weight `tie_w`.  Thread t has the bins 2 t and 2 t + 1.
+  // entries of weight `tie_w`.  Thread t has kPer bins, from kPer t on.
   template <bool W, typename F>
   __device__ void find(F need_of, int tie_bin, uint64_t tie_n, uint64_t tie_w) {
-    uint64_t n[2] = {0, 0}, v[2] = {0, 0};
+    uint64_t n[kPer] = {}, v[kPer] = {};
     for (int r = 0; r < ranks; ++r) {
       const Shared* o = cluster.map_shared_rank(&sm, r);
-      const uint2 q = reinterpret_cast<const uint2*>(o->cnt[buf])[tid];
-      n[0] += q.x;
-      n[1] += q.y;
-      if (W) {
-        const uint2 l = reinterpret_cast<const uint2*>(o->lo[buf])[tid], h = reinterpret_cast<const uint2*>(o->hi[buf])[tid];
-        v[0] += (uint64_t)l.x + ((uint64_t)h.x << 32);
-        v[1] += (uint64_t)l.y + ((uint64_t)h.y << 32);
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        const uint2 q = *reinterpret_cast<const uint2*>(o->cnt[buf] + kPer * tid + e);
+        n[e] += q.x;
+        n[e + 1] += q.y;
+        if (W) {
+          const uint2 l = *reinterpret_cast<const uint2*>(o->lo[buf] + kPer * tid + e);
+          const uint2 h = *reinterpret_cast<const uint2*>(o->hi[buf] + kPer * tid + e);
+          v[e] += (uint64_t)l.x + ((uint64_t)h.x << 32);
+          v[e + 1] += (uint64_t)l.y + ((uint64_t)h.y << 32);
+        }
       }
     }
+    uint64_t mine = 0;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (2 * tid + e == tie_bin) {
+    for (int e = 0; e < kPer; ++e) {
+      if (kPer * tid + e == tie_bin) {
         n[e] += tie_n;
         v[e] += tie_n * tie_w;
       }
       if (!W) v[e] = n[e];
+      mine += v[e];
     }
-    uint64_t inc = v[0] + v[1];
+    uint64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
@@ -266,11 +340,11 @@ struct Row {
     inc += before;
     if (tid == 0) sm.found_total = total;
     const uint64_t need = need_of(total);
-    uint64_t at = inc - v[0] - v[1];
+    uint64_t at = inc - mine;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < kPer; ++e) {
       if (at < need && at + v[e] >= need) {
-        sm.found = (uint32_t)(2 * tid + e);
+        sm.found = (uint32_t)(kPer * tid + e);
         sm.found_cnt = (uint32_t)n[e];
         sm.found_above = at;
       }
@@ -280,7 +354,7 @@ struct Row {
   }
 
   __device__ void clear_hist(int b) {
-    for (int i = tid; i < kBins; i += kThreads) sm.cnt[b][i] = sm.lo[b][i] = sm.hi[b][i] = 0;
+    for (int i = tid; i < kBins; i += NT) sm.cnt[b][i] = sm.lo[b][i] = sm.hi[b][i] = 0;
   }
 
   template <bool W>
@@ -370,19 +444,19 @@ struct Row {
     for (int r = 0; r < ranks; ++r) {
       const Shared* o = cluster.map_shared_rank(&sm, r);
       const uint32_t m = min(o->list_n, (uint32_t)kList);
-      for (uint32_t i = tid; i < m && total + i < (uint32_t)kCand; i += kThreads) sm.keys[total + i] = o->list[i];
+      for (uint32_t i = tid; i < m && total + i < (uint32_t)kCand; i += NT) sm.keys[total + i] = o->list[i];
       total += m;
     }
     if (tie_in && tid == 0 && total < (uint32_t)kCand) sm.keys[total] = tie_key;
     if (tie_in) ++total;
     total = min(total, (uint32_t)kCand);
     __syncthreads();
-    for (uint32_t i = tid; i < total; i += kThreads) {
+    for (uint32_t i = tid; i < total; i += NT) {
       const uint64_t w = W ? weight(value_of(sm.keys[i])) : 1;
       sm.weights[i] = (tie_in && i == total - 1) ? ties * w : w;
     }
     __syncthreads();
-    for (uint32_t i0 = 0; i0 < total; i0 += kThreads / kLanes) {
+    for (uint32_t i0 = 0; i0 < total; i0 += NT / kLanes) {
       const uint32_t i = i0 + tid / kLanes;
       const uint32_t k = i < total ? sm.keys[i] : 0;
       uint64_t gt = 0, eq = 0;
@@ -422,32 +496,38 @@ struct Row {
     each<kAhead>([&](int, float v) {
       const float t = (top - v) * c;
       if (!(t < (float)kBins)) return;  // NaN, and what weighs nothing
-      const int b = (int)t;
-      atomicAdd(&sm.cnt[buf][b], 1u);
-      atomicAdd(&sm.lo[buf][b], (uint32_t)((t - (float)b) * 4096.0f));
+      const uint32_t fixed = (uint32_t)(t * 4096.0f);
+      atomicAdd(&sm.cnt[buf][fixed >> 12], 1u);
+      atomicAdd(&sm.lo[buf][fixed >> 12], fixed & 4095u);
     });
     if (tid == 0) sm.list_n = 0;
     cluster.sync();
-    uint64_t n[2] = {0, 0}, f[2] = {0, 0};
+    uint64_t n[kPer] = {}, f[kPer] = {};
     for (int r = 0; r < ranks; ++r) {
       const Shared* o = cluster.map_shared_rank(&sm, r);
-      const uint2 q = reinterpret_cast<const uint2*>(o->cnt[buf])[tid], g = reinterpret_cast<const uint2*>(o->lo[buf])[tid];
-      n[0] += q.x;
-      n[1] += q.y;
-      f[0] += g.x;
-      f[1] += g.y;
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        const uint2 q = *reinterpret_cast<const uint2*>(o->cnt[buf] + kPer * tid + e);
+        const uint2 g = *reinterpret_cast<const uint2*>(o->lo[buf] + kPer * tid + e);
+        n[e] += q.x;
+        n[e + 1] += q.y;
+        f[e] += g.x;
+        f[e + 1] += g.y;
+      }
     }
     // the lower bounds in units of 2^-40 of the largest weight: whole numbers again, so that
     // every CTA finds the same bins
-    uint64_t w[2], inc[2] = {0, 0};
+    uint64_t w[kPer], inc[2] = {0, 0}, mine[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      w[e] = n[e] ? (uint64_t)((double)n[e] * exp(-kStep * ((double)(2 * tid + e) + (double)f[e] / (4096.0 * (double)n[e]))) *
+    for (int e = 0; e < kPer; ++e) {
+      w[e] = n[e] ? (uint64_t)((double)n[e] * exp(-kStep * ((double)(kPer * tid + e) + (double)f[e] / (4096.0 * (double)n[e]))) *
                                1099511627776.0)
                   : 0;
       inc[0] += w[e];
       inc[1] += n[e];
     }
+    mine[0] = inc[0];
+    mine[1] = inc[1];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
@@ -470,15 +550,15 @@ struct Row {
     }
     const double part = (double)p * (double)all;
     const uint64_t low = max((uint64_t)1, (uint64_t)(part * 0.9996)), high = max(low, min(all, (uint64_t)(part * 1.0004) + 1));
-    uint64_t at = inc[0] - w[0] - w[1], many = inc[1] - n[0] - n[1];
+    uint64_t at = inc[0] - mine[0], many = inc[1] - mine[1];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < kPer; ++e) {
       if (at < low && at + w[e] >= low) {
-        sm.found = (uint32_t)(2 * tid + e);
+        sm.found = (uint32_t)(kPer * tid + e);
         sm.found_above = many;
       }
       if (at < high && at + w[e] >= high) {
-        sm.found_cnt = (uint32_t)(2 * tid + e);
+        sm.found_cnt = (uint32_t)(kPer * tid + e);
         sm.found_total = many + n[e];
       }
       at += w[e];
@@ -553,7 +633,7 @@ struct Row {
   __device__ void among(int n, int k, float p, uint64_t least, float u, int row) {
     const int most = min(n, k);
     // ranks, and the weights in order of rank
-    for (int i0 = 0; i0 < n; i0 += kThreads / kLanes) {
+    for (int i0 = 0; i0 < n; i0 += NT / kLanes) {
       const int i = i0 + tid / kLanes;
       const uint32_t key = i < n ? sm.keys[i] : 0, id = i < n ? sm.idx[i] : 0;
       uint32_t place = 0;
@@ -570,9 +650,14 @@ struct Row {
       }
     }
     __syncthreads();
-    uint64_t w[2] = {2 * tid < most ? sm.weights[2 * tid] : 0, 2 * tid + 1 < most ? sm.weights[2 * tid + 1] : 0};
+    uint64_t w[kPer], mine = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      w[e] = kPer * tid + e < most ? sm.weights[kPer * tid + e] : 0;
+      mine += w[e];
+    }
     if (p < 1.0f) {  // in order of rank, those before which `enough` is not reached yet
-      uint64_t inc = w[0] + w[1];
+      uint64_t inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
@@ -580,24 +665,30 @@ struct Row {
       }
       if (lane == 31) sm.red[warp] = inc;
       __syncthreads();
-      uint64_t before = inc - w[0] - w[1], total = 0;
+      uint64_t before = inc - mine, total = 0;
       for (int e = 0; e < kWarps; ++e) {
         if (e < warp) before += sm.red[e];
         total += sm.red[e];
       }
       const uint64_t enough = nucleus(p, total);
-      if (before + w[0] >= enough) w[1] = 0;
-      if (before >= enough) w[0] = 0;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const uint64_t next = before + w[e];
+        if (before >= enough) w[e] = 0;
+        before = next;
+      }
       __syncthreads();
     }
+    mine = 0;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < kPer; ++e) {
       if (w[e] < least) w[e] = 0;
-      if (2 * tid + e < n) sm.weights[2 * tid + e] = w[e];
+      mine += w[e];
+      if (kPer * tid + e < n) sm.weights[kPer * tid + e] = w[e];
     }
-    const uint64_t at = drawn(u, block_sum(w[0] + w[1], sm.red));
+    const uint64_t at = drawn(u, block_sum(mine, sm.red));
     // the pick, in index order
-    for (int i0 = 0; i0 < n; i0 += kThreads / kLanes) {
+    for (int i0 = 0; i0 < n; i0 += NT / kLanes) {
       const int i = i0 + tid / kLanes;
       const uint32_t id = i < n ? sm.idx[i] : 0;
       uint64_t before = 0;
@@ -617,23 +708,12 @@ struct Row {
     const float mp = a.min_p ? a.min_p[row] : 0.0f;
     const float u = a.u[row];
     float mine = -INFINITY;
-    int mine_i = -1;
-    each<kAhead>([&](int i, float v) {
-      if (v > mine) {  // a lane meets its entries in index order
-        mine = v;
-        mine_i = i;
-      }
-    });
-    if (mine_i < 0) {  // nothing above -inf: its first -inf, if any
-      each<1>([&](int i, float v) {
-        if (v == -INFINITY && mine_i < 0) mine_i = i;
-      });
-    }
-    uint64_t best = mine_i >= 0 ? ((uint64_t)key_of(mine) << 32) | (0xffffffffu - (uint32_t)mine_i) : 0;
+    each_max([&](float v) { mine = fmaxf(mine, v); });
+    uint64_t best = key_of(mine);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (lane == 0) sm.red[warp] = best;
-    if (tid == 0) sm.cand_n = 0;
+    if (tid == 0) sm.cand_n = 0, sm.first = 0x7fffffffu;
     if (tid < 64) sm.pow2[tid] = exp2(44.0 - (double)tid / 64.0);
     buf = 0;
     clear_hist(0);
@@ -648,9 +728,16 @@ struct Row {
     cluster.sync();
     best = 0;
     for (int r = 0; r < ranks; ++r) best = max(best, cluster.map_shared_rank(&sm, r)->xch[0][0]);
-    top = value_of((uint32_t)(best >> 32));
-    if (best == 0 || !(fabsf(top) < INFINITY) || !(t > 0.0f) || k == 1) {
-      if (rank == 0 && tid == 0) a.ids[row] = best == 0 ? 0 : (int)(0xffffffffu - (uint32_t)best);
+    top = value_of((uint32_t)best);
+    if (!(fabsf(top) < INFINITY) || !(t > 0.0f) || k == 1) {  // the maximum's lowest index
+      uint32_t first = 0x7fffffffu;
+      each_from(top, [&](int i, float v) {
+        if (v == top) first = min(first, (uint32_t)i);
+      });
+      first = __reduce_min_sync(0xffffffffu, first);
+      if (lane == 0) atomicMin(&cluster.map_shared_rank(&sm, 0)->first, first);
+      cluster.sync();
+      if (rank == 0 && tid == 0) a.ids[row] = sm.first == 0x7fffffffu ? 0 : (int)sm.first;  // NaN alone: 0
       return;
     }
     topd = (double)top;
@@ -664,7 +751,7 @@ struct Row {
       // The lanes' maxima bound the k-th largest from below: at least k entries lie in the
       // bins up to the one where the maxima reach k, and with many more lanes than k few
       // others do.
-      bool few = 2 * k <= ranks * kThreads;
+      bool few = 2 * k <= ranks * NT;
       if (few) {
         if (mine > -INFINITY) atomicAdd(&sm.cnt[0][bin(mine)], 1u);
         cluster.sync();
@@ -676,7 +763,9 @@ struct Row {
       if (few) {
         const float upto = (float)(sm.found + 1);
         Shared* o = cluster.map_shared_rank(&sm, 0);
-        each<kAhead>([&](int i, float v) {
+        // a little below the last value that qualifies: the exact test follows
+        const float from = top - upto / c - 1e-5f * (upto / c + fabsf(top));
+        each_from(from, [&](int i, float v) {
           if (!((top - v) * c < upto)) return;
           const uint32_t at = atomicAdd(&o->cand_n, 1u);
           if (at < (uint32_t)kCand) {
@@ -802,36 +891,38 @@ struct Row {
   }
 };
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sm = *reinterpret_cast<Shared*>(smem);
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = (int)(blockIdx.x / ranks);
   const int tid = threadIdx.x, warp = tid >> 5;
-  const int64_t first = (int64_t)(rank * kWarps + warp) * a.per_warp;
+  const int64_t first = (int64_t)(rank * (NT / 32) + warp) * a.per_warp;
   constexpr int es = DT == 0 ? 4 : 2;
-  Row<DT> r{a, sm, cluster, static_cast<const uint8_t*>(a.x) + (int64_t)row * a.ldx * es, rank, ranks, tid, tid & 31, warp,
-            (int)min(first, (int64_t)a.V), (int)min(first + a.per_warp, (int64_t)a.V)};
+  Row<DT, NT> r{a, sm, cluster, static_cast<const uint8_t*>(a.x) + (int64_t)row * a.ldx * es, rank, ranks, tid, tid & 31, warp,
+                (int)min(first, (int64_t)a.V), (int)min(first + a.per_warp, (int64_t)a.V)};
   r.run(row);
   cluster.sync();  // no CTA leaves while another may read its shared memory
 }
 
-template <int DT>
-cudaError_t sample_launch(const SampleArgs& a, int64_t T, int ranks, cudaStream_t st) {
+template <int DT, int NT>
+cudaError_t sample_launch(SampleArgs a, int64_t T, int ranks, cudaStream_t st) {
   static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (!(configured.load(std::memory_order_relaxed) & bit)) {
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel<DT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit, std::memory_order_relaxed);
   }
+  const int64_t warps = (int64_t)ranks * (NT / 32);
+  a.per_warp = (int)((a.V + warps - 1) / warps + 255) / 256 * 256;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(T * ranks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -841,7 +932,7 @@ cudaError_t sample_launch(const SampleArgs& a, int64_t T, int ranks, cudaStream_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, sample_kernel<DT>, a);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<DT, NT>, a);
 }
 
 }  // namespace
@@ -850,13 +941,12 @@ cudaError_t launch_sample(const void* x, int dt, int64_t ldx, int64_t T, int64_t
                           const int* top_k, const float* top_p, const float* min_p, const float* u, int* ids,
                           cudaStream_t st) {
   if (T <= 0) return cudaSuccess;
-  int ranks = 1;
-  while (ranks < kMaxRanks && V > (int64_t)ranks * 8 * kThreads && 2 * ranks * T <= kResident) ranks *= 2;
-  const int64_t warps = (int64_t)ranks * kWarps;
   const int es = dt == 0 ? 4 : 2;
   const int wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (T == 1 || ldx * es % 16 == 0);
-  SampleArgs a{x, ldx, (int)V, (int)(((V + warps - 1) / warps + 255) / 256 * 256), wide, temperature, top_k, top_p, min_p, u, ids};
-  return dt == 0 ? sample_launch<0>(a, T, ranks, st) : dt == 1 ? sample_launch<1>(a, T, ranks, st) : sample_launch<2>(a, T, ranks, st);
+  const SampleArgs a{x, ldx, (int)V, 0, wide, temperature, top_k, top_p, min_p, u, ids};
+  int ranks = 1;
+  while (ranks < kMaxRanks && V > (int64_t)ranks * 4096 && 2 * ranks * T <= kResident) ranks *= 2;
+  return dt == 0 ? sample_launch<0, kNT>(a, T, ranks, st) : dt == 1 ? sample_launch<1, kNT>(a, T, ranks, st) : sample_launch<2, kNT>(a, T, ranks, st);
 }
 
 }  // namespace rtd
