@@ -4,7 +4,8 @@
     python -m runtimed_b200.build --force    # rebuild everything
 
 Each source compiles to an object under runtimed_b200/_build/ (git-ignored);
-the shared library lands next to this file so it travels with the tree.
+the shared library lands next to this file so it travels with the tree, and beside
+it _rtd_torch.so, the binding that hands torch tensors to it (csrc/rtd_torch.cpp).
 """
 from __future__ import annotations
 
@@ -20,6 +21,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libruntimed_b200.so")
+TORCH_LIB = os.path.join(HERE, "_rtd_torch.so")
 INCLUDE = os.path.join(ROOT, "include")
 
 SOURCES = ["rtd_api.cu", "rtd_gemv.cu", "rtd_gemm.cu", "rtd_gemm_ts.cu", "rtd_tp.cu", "rtd_model.cu", "rtd_kv4.cu",
@@ -76,7 +78,28 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force or _stale(LIB, objs):
         cmd = [nvcc(), "-ccbin", host_cxx(), *ARCH, "-shared", "-o", LIB, *objs, "-cudart", "static"]
         subprocess.run(cmd, check=True)
+    torch_binding(force)
     return LIB
+
+
+def torch_binding(force: bool = False) -> str:
+    """_rtd_torch.so next to the library: torch tensors into the C ABI (csrc/rtd_torch.cpp)."""
+    import sysconfig
+
+    src = os.path.join(CSRC, "rtd_torch.cpp")
+    if not force and not _stale(TORCH_LIB, [src, os.path.join(INCLUDE, "rtd.h")]):
+        return TORCH_LIB
+    import torch
+    from torch.utils import cpp_extension as ext
+
+    inc = [f"-isystem{d}" for d in ext.include_paths() + [sysconfig.get_paths()["include"], "/usr/local/cuda/include"]]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [host_cxx(), "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", *inc, src, "-o", TORCH_LIB,
+           f"-L{HERE}", "-l:libruntimed_b200.so", f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN"]
+    subprocess.run(cmd, check=True)
+    return TORCH_LIB
 
 
 def main() -> int:

@@ -17,6 +17,7 @@ weight is moved to the weight's device first, as the reference does with
 from __future__ import annotations
 
 import ctypes
+import sys
 from typing import Dict, Optional
 
 import numpy as np
@@ -74,6 +75,9 @@ class Context:
 
     def close(self) -> None:
         if self.handle:
+            torch_binding = sys.modules.get(f"{__package__}._torch")
+            if torch_binding is not None and Context._by_device.get(self.device.index) is self:
+                torch_binding.binding.forget(self.device.index)  # it keeps the address
             _lib.lib().rtd_destroy(self.handle)
             self.handle = None
 
