@@ -36,6 +36,18 @@ namespace {
 
 constexpr int kTok = 16;  // tokens of a page
 
+// The kernel's shared-memory limit, set once per device (a bit each in `configured`).
+template <typename K>
+cudaError_t configure_once(K kernel, int smem, std::atomic<uint64_t>& configured) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e != cudaSuccess || (configured.load(std::memory_order_relaxed) & bit)) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) configured.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 __device__ __forceinline__ float load_as_f32(const void* p, int dt, int64_t i) {
   if (dt == 0) return static_cast<const float*>(p)[i];
   if (dt == 1) return __half2float(static_cast<const __half*>(p)[i]);
@@ -1112,15 +1124,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) kv4_attn_kernel(cons
 template <int NG, bool EXACT>
 cudaError_t attn_launch(Kv4AttnArgs a, int sm_count, cudaStream_t st) {
   constexpr int smem = Attn<NG, EXACT>::kSmem;
-  static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(configured.load(std::memory_order_relaxed) & bit)) {
-    cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<NG, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    configured.fetch_or(bit, std::memory_order_relaxed);
-  }
+  static std::atomic<uint64_t> configured{0};
+  cudaError_t e = configure_once(kv4_attn_kernel<NG, EXACT>, smem, configured);
+  if (e != cudaSuccess) return e;
   // never more CTAs than the bounds on the lengths can give work to
   const int64_t tiles = ((int64_t)a.max_q * (a.n_head / a.n_kv) + kRows - 1) / kRows;
   const double most = (double)a.S * a.n_kv * tiles * (kUnitCost + (a.max_ctx + kTok - 1) / kTok);
@@ -1139,11 +1145,16 @@ cudaError_t launch_kv_plan(const int* want, int S, int* length, int* table, int 
   PlanArgs a{want, S, length, table, max_blocks, free_list, free_count, num_blocks, q_start, tok_seq, tok_pos,
              tok_slot, max_tokens, status};
   const size_t smem = (size_t)(4 * S + 3) * sizeof(int);
-  cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (4 * kPlanMaxSeqs + 3) * (int)sizeof(int));
+  static std::atomic<uint64_t> configured{0};
+  cudaError_t e = configure_once(kv_plan_kernel, (4 * kPlanMaxSeqs + 3) * (int)sizeof(int), configured);
   if (e != cudaSuccess) return e;
   const int64_t items = (q_start ? max_tokens : 0) + (int64_t)S;
   const unsigned ctas = items > 4 * kPlanThreads ? 8 : 1;
+  count_launch();
+  if (ctas == 1) {
+    kv_plan_kernel<<<1, kPlanThreads, smem, st>>>(a);
+    return cudaGetLastError();
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kPlanThreads);
@@ -1155,7 +1166,6 @@ cudaError_t launch_kv_plan(const int* want, int S, int* length, int* table, int 
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  count_launch();
   return cudaLaunchKernelEx(&cfg, kv_plan_kernel, a);
 }
 

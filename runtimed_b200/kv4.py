@@ -85,3 +85,54 @@ def _code(dtype: torch.dtype) -> int:
     if code is None:
         raise ConfigError(f"{dtype} (f32, f16 or bf16)")
     return code
+
+
+class BlockTables:
+    """Device-side bookkeeping of a paged cache: lengths, block table and free stack, and the
+    token lists of a step, in buffers of their own (a step may be captured in a CUDA graph).
+
+    ``from_cache`` takes over the state of a host-side ``PagedKvCache`` and ``into`` gives it
+    back; between the two the host's copy is stale."""
+
+    def __init__(self, max_seqs: int, max_blocks: int, num_blocks: int, max_tokens: int, device="cuda:0"):
+        if not 0 < max_seqs <= MAX_SEQS:
+            raise ConfigError(f"block tables of {max_seqs} sequences (1 to {MAX_SEQS})")
+        i32 = dict(dtype=torch.int32, device=device)
+        self.length = torch.zeros((max_seqs,), **i32)
+        self.table = torch.zeros((max_seqs, max_blocks), **i32)
+        self.free_list = torch.arange(num_blocks - 1, -1, -1, **i32)
+        self.free_count = torch.full((1,), num_blocks, **i32)
+        self.q_start = torch.zeros((max_seqs + 1,), **i32)
+        self.tok_seq, self.tok_pos, self.tok_slot = (torch.full((max_tokens,), -1, **i32) for _ in range(3))
+
+    def step(self, want: torch.Tensor) -> None:
+        """Sequences to ``want`` tokens (int32 [max_seqs]); the new tokens into q_start / tok_*."""
+        plan(want, self.length, self.table, self.free_list, self.free_count,
+             out=(self.q_start, self.tok_seq, self.tok_pos, self.tok_slot))
+
+    def set_lengths(self, want: torch.Tensor) -> None:
+        """The same without token lists (a rollback, a release)."""
+        plan(want, self.length, self.table, self.free_list, self.free_count)
+
+    @classmethod
+    def from_cache(cls, cache, max_tokens: int) -> "BlockTables":
+        t = cls(cache.max_seqs, cache.max_blocks, cache.num_blocks, max_tokens, cache.device)
+        length = np.zeros(cache.max_seqs, np.int32)
+        for s, n in cache.lengths.items():
+            length[s] = n
+        free = np.zeros(cache.num_blocks, np.int32)
+        free[:len(cache._free)] = cache._free
+        t.length.copy_(torch.from_numpy(length))
+        t.table.copy_(torch.from_numpy(cache._host_table))
+        t.free_list.copy_(torch.from_numpy(free))
+        t.free_count.fill_(len(cache._free))
+        return t
+
+    def into(self, cache) -> None:
+        """The state back to the host's cache (waits for the device)."""
+        length, table = self.length.cpu().numpy(), self.table.cpu().numpy()
+        cache._free = self.free_list[:int(self.free_count)].tolist()
+        cache._host_table[:] = table
+        cache._blocks = {s: table[s, :-(-int(n) // BLOCK)].tolist() for s, n in enumerate(length) if n}
+        cache.lengths = {s: int(n) for s, n in enumerate(length) if n}
+        cache._dirty = True

@@ -5,14 +5,17 @@ with the model's arithmetic in libruntimed_b200.so: ``rtd_qembed`` for the embed
 ``rtd_qlinear`` for every linear (bias fused), and the decoder-layer operations
 ``rtd_rmsnorm`` (residual add fused), ``rtd_rope_kv_append``, ``rtd_attention_paged``,
 ``rtd_silu_mul`` and ``rtd_argmax``.  The residual stream and every linear's input and
-output are f32, as in the reference's CPU path; the KV cache is f16 and PAGED
-(``PagedKvCache``: 16-token blocks from one pool, a block table per sequence,
+output are f32, as in the reference's CPU path; the KV cache is f16 (or f32, or 4 bits:
+``kv_dtype="q4"``, runtimed_b200.kv4) and PAGED (``PagedKvCache``: 16-token blocks from
+one pool, a block table per sequence,
 crates/runtimed-model/src/cache/paged/table.rs:57-145), which the reference leaves
 unwired for Qwen2 (its forward is batch-1 over a contiguous cache).  Every token of a
 call carries its own (sequence, position), so ``forward`` serves a prefill chunk of one
 sequence, ``decode_batch`` one token of many sequences, and a speculative verify of
 k + 1 positions followed by ``PagedKvCache.truncate`` (the rollback of rejected
-positions, crates/runtimed-model/src/decode/speculate.rs:31-199).
+positions, crates/runtimed-model/src/decode/speculate.rs:31-199).  ``generate_batch``
+samples for many sequences with the whole step on the device (block tables, layers,
+sampling) in one captured graph.
 
 With a communicator (one process per GPU) the decoder runs tensor parallel over N ranks,
 the reference's dual-GPU blocks (crates/runtimed-model/src/tp/dual_gpu.rs:52-186,
@@ -31,7 +34,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Union
 
 import numpy as np
 import torch
@@ -89,22 +92,30 @@ class Qwen2Config:
 
 
 class PagedKvCache:
-    """f16 K / V of every layer in 16-token blocks from one pool, with a block table per
-    sequence.  Block ids come from a free list; ``reserve`` grows a sequence to a length,
+    """f16 K / V of every layer in 16-token blocks from one pool (``dtype`` f32, or "q4" for
+    4-bit pages: ``pages`` instead of ``k`` and ``v``), with a block table per sequence.
+    Block ids come from a free list; ``reserve`` grows a sequence to a length,
     ``truncate`` shrinks it (blocks past the new length return to the pool), ``release``
     frees it."""
 
     def __init__(self, cfg: Qwen2Config, num_blocks: int, max_seqs: int, max_ctx: int, device,
-                 dtype: torch.dtype = torch.float16):
-        if dtype not in (torch.float16, torch.float32):
-            raise ConfigError(f"KV cache dtype {dtype} (f16 or f32)")
+                 dtype: Union[torch.dtype, str] = torch.float16):
+        if dtype not in (torch.float16, torch.float32, "q4"):
+            raise ConfigError(f"KV cache dtype {dtype} (f16, f32 or \"q4\")")
         self.cfg, self.device, self.dtype = cfg, torch.device(device), dtype
-        self.abi_dtype = _lib.DT_F16 if dtype == torch.float16 else _lib.DT_F32
+        self.q4 = dtype == "q4"
+        self.abi_dtype = _lib.DT_F32 if dtype == torch.float32 else _lib.DT_F16
         self.num_blocks, self.max_seqs = int(num_blocks), int(max_seqs)
         self.max_blocks = -(-int(max_ctx) // KV_BLOCK)
-        shape = (self.num_blocks, cfg.n_kv, KV_BLOCK, cfg.head_dim)
-        self.k = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(cfg.n_layer)]
-        self.v = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(cfg.n_layer)]
+        if self.q4:
+            from . import kv4
+
+            self.pages = [kv4.alloc_pages(self.num_blocks, cfg.n_kv, cfg.head_dim, self.device) for _ in range(cfg.n_layer)]
+            self.k = self.v = []
+        else:
+            shape = (self.num_blocks, cfg.n_kv, KV_BLOCK, cfg.head_dim)
+            self.k = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(cfg.n_layer)]
+            self.v = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(cfg.n_layer)]
         self.table = torch.zeros((self.max_seqs, self.max_blocks), dtype=torch.int32, device=self.device)
         self._host_table = np.zeros((self.max_seqs, self.max_blocks), dtype=np.int32)
         self._free: List[int] = list(range(self.num_blocks - 1, -1, -1))
@@ -141,24 +152,54 @@ class PagedKvCache:
         self._blocks.pop(seq, None)
         self.lengths.pop(seq, None)
 
+    def slots(self, seqs: Sequence[int], positions: Sequence[int]) -> np.ndarray:
+        """int32 slots (block * 16 + offset) of reserved (sequence, position) pairs."""
+        s, p = np.asarray(seqs, dtype=np.int64), np.asarray(positions, dtype=np.int64)
+        return (self._host_table[s, p // KV_BLOCK] * KV_BLOCK + p % KV_BLOCK).astype(np.int32)
+
+    def values(self, layer: int, seq: int, dtype: torch.dtype = torch.float32):
+        """(k, v) [length, n_kv, head_dim] that layer `layer` holds of a sequence: what
+        attention sees, whatever the cache's type."""
+        n = self.lengths.get(seq, 0)
+        slots = torch.from_numpy(self.slots([seq] * n, range(n))).to(self.device)
+        if self.q4:
+            from . import kv4
+
+            return kv4.read(self.pages[layer], slots, dtype)
+        at = slots.long()
+        return tuple(c[layer][at // KV_BLOCK, :, at % KV_BLOCK].to(dtype) for c in (self.k, self.v))
+
     def sync_table(self) -> None:
         if self._dirty:
             self.table.copy_(torch.from_numpy(self._host_table))
             self._dirty = False
 
 
+@dataclass
+class _Q4Step:
+    """What the 4-bit cache's kernels need of a call's tokens, on the device: their slots, and
+    for each row of `table` its queries' offsets and its length after the call."""
+
+    slot: torch.Tensor
+    q_start: torch.Tensor
+    ctx_len: torch.Tensor
+    table: torch.Tensor
+    max_q: int
+
+
 class Qwen2Model:
     """Weights on one device and the forward over a paged KV cache.
 
     ``kv_dtype`` is the cache precision (f16 by default, as the configs run; f32 is the
-    reference CPU cache's precision).  ``exact_linears`` runs every linear through the
+    reference CPU cache's precision; "q4" holds keys and values in 4 bits, in 5 / 16 of the
+    f16 cache's memory).  ``exact_linears`` runs every linear through the
     decode GEMV in passes of at most three tokens, whose products are exact (f32 rounding
     only), instead of the tensor-core GEMM, whose f16-rounded weights cost about 3e-4
     relative per linear; the parity checks use it to separate the layer math from the
     GEMM's rounding, which peaked attention over a long prompt amplifies."""
 
     def __init__(self, path_or_file, device="cuda:0", max_seqs: int = 1, max_ctx: int = 4096,
-                 kv_blocks: Optional[int] = None, kv_dtype: torch.dtype = torch.float16,
+                 kv_blocks: Optional[int] = None, kv_dtype: Union[torch.dtype, str] = torch.float16,
                  exact_linears: bool = False, comm=None):
         self.file = path_or_file if isinstance(path_or_file, GgufFile) else GgufFile.open(path_or_file)
         self.cfg = Qwen2Config.from_gguf(self.file)
@@ -180,6 +221,10 @@ class Qwen2Model:
         self.cache = PagedKvCache(local, blocks, max_seqs, max_ctx, self.device, kv_dtype)
         self.max_ctx = int(max_ctx)
         self.exact_linears = bool(exact_linears)
+        if self.cache.q4:
+            from . import kv4
+
+            self.inv_freq = kv4.rope_frequencies(cfg.head_dim, cfg.rope_theta, self.device)
 
     # ---- load (crates/runtimed-model/src/weights/load_gguf.rs:47-120)
     FUSE = (("qkv", ("attn_q", "attn_k", "attn_v")), ("gate_up", ("ffn_gate", "ffn_up")))
@@ -293,10 +338,15 @@ class Qwen2Model:
     # ---- one call over T tokens, each with its own (sequence, position)
     def _run(self, ids: torch.Tensor, tok_seq: torch.Tensor, tok_pos: torch.Tensor, max_ctx: int,
              logits_rows: Optional[torch.Tensor] = None, trace: Optional[list] = None,
-             head_ids: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+             head_ids: Optional[torch.Tensor] = None, q4: Optional[_Q4Step] = None,
+             block_table: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """Logits of the call's tokens (rows `logits_rows` only, when given); with `head_ids`
         (int32 [rows]) the greedy ids are written there instead, the pick fused into the LM
-        head (rtd_qlinear_argmax: no logits written below four rows), and None is returned."""
+        head (rtd_qlinear_argmax: no logits written below four rows), and None is returned.
+        `q4` comes with a 4-bit cache; `block_table` stands for the cache's own where given."""
+        if self.cache.q4:
+            from . import kv4
+
         cfg, L, st = self.cfg, self.L, _stream_ptr(self.device)
         T = int(ids.shape[0])
         c = self.ctx.handle
@@ -317,6 +367,7 @@ class Qwen2Model:
             fq = self.fused.get((i, "qkv"))
             if fq is not None:  # q | k | v from one launch: column slices of one output
                 qkv = self._lin(n, cfg.hidden, T, fq[0], fq[1])
+                q, k, v = qkv.split(fq[2], 1)
                 w = qkv.shape[1]
                 qp, kp = qkv.data_ptr(), qkv.data_ptr() + 4 * fq[2][0]
                 vp = kp + 4 * fq[2][1]
@@ -327,16 +378,23 @@ class Qwen2Model:
                 k = self._linear(n, f"{p}.attn_k.weight", f"{p}.attn_k.bias" if bias else None)
                 v = self._linear(n, f"{p}.attn_v.weight", f"{p}.attn_v.bias" if bias else None)
                 qp, kp, vp, ldq, ldk, ldv = q.data_ptr(), k.data_ptr(), v.data_ptr(), q.shape[1], k.shape[1], v.shape[1]
-            self._check(L.rtd_rope_kv_append(c, qp, ldq, kp, ldk, vp, ldv, T, nh, nkv, cfg.head_dim,
-                                             cfg.head_dim, cfg.rope_theta, tok_seq.data_ptr(), tok_pos.data_ptr(),
-                                             self.cache.table.data_ptr(), self.cache.max_blocks,
-                                             self.cache.k[i].data_ptr(), self.cache.v[i].data_ptr(),
-                                             self.cache.abi_dtype, qr.data_ptr(), st))
-            self._check(L.rtd_attention_paged(c, qr.data_ptr(), T, nh, nkv, cfg.head_dim, scale,
-                                              tok_seq.data_ptr(), tok_pos.data_ptr(), self.cache.table.data_ptr(),
-                                              self.cache.max_blocks, max_ctx, self.cache.k[i].data_ptr(),
-                                              self.cache.v[i].data_ptr(), self.cache.abi_dtype, att.data_ptr(),
-                                              _lib.DT_F32, att.shape[1], st))
+            if self.cache.q4:
+                by_head = [x.unflatten(1, (h, cfg.head_dim)) for x, h in ((q, nh), (k, nkv), (v, nkv), (qr, nh), (att, nh))]
+                kv4.append(*by_head[:3], self.inv_freq, tok_pos, q4.slot, self.cache.pages[i], by_head[3])
+                kv4.attention(by_head[3], self.cache.pages[i], q4.table, q4.q_start, q4.ctx_len, q4.max_q, max_ctx,
+                              scale, out=by_head[4])
+            else:
+                table = self.cache.table if block_table is None else block_table
+                self._check(L.rtd_rope_kv_append(c, qp, ldq, kp, ldk, vp, ldv, T, nh, nkv, cfg.head_dim,
+                                                 cfg.head_dim, cfg.rope_theta, tok_seq.data_ptr(), tok_pos.data_ptr(),
+                                                 table.data_ptr(), self.cache.max_blocks,
+                                                 self.cache.k[i].data_ptr(), self.cache.v[i].data_ptr(),
+                                                 self.cache.abi_dtype, qr.data_ptr(), st))
+                self._check(L.rtd_attention_paged(c, qr.data_ptr(), T, nh, nkv, cfg.head_dim, scale,
+                                                  tok_seq.data_ptr(), tok_pos.data_ptr(), table.data_ptr(),
+                                                  self.cache.max_blocks, max_ctx, self.cache.k[i].data_ptr(),
+                                                  self.cache.v[i].data_ptr(), self.cache.abi_dtype, att.data_ptr(),
+                                                  _lib.DT_F32, att.shape[1], st))
             o = self._row(att, att.shape[1], T, self.weights.q_map[f"{p}.attn_output.weight"])
             self._check(L.rtd_rmsnorm(c, h.data_ptr(), cfg.hidden, o.data_ptr(), _lib.DT_F32, cfg.hidden,
                                       self.weights.map[f"{p}.ffn_norm.weight"].data_ptr(), cfg.eps, T, cfg.hidden,
@@ -388,14 +446,23 @@ class Qwen2Model:
         seq_d = self._tokens([seq] * t)
         pos_d = self._tokens(range(q0, q0 + t))
         rows = self._tokens([t - 1]) if last_only else None
-        return self._run(ids_d, seq_d, pos_d, q0 + t, rows, trace)
+        q4 = None
+        if self.cache.q4:
+            q4 = _Q4Step(self._tokens(self.cache.slots([seq] * t, range(q0, q0 + t))), self._tokens([0, t]),
+                         self._tokens([q0 + t]), self.cache.table[seq:seq + 1], t)
+        return self._run(ids_d, seq_d, pos_d, q0 + t, rows, trace, q4=q4)
 
     def decode_batch(self, ids: Sequence[int], seqs: Sequence[int], positions: Sequence[int]) -> torch.Tensor:
         """One token for each of several sequences (batched decode); logits [b, vocab]."""
         for s, p in zip(seqs, positions):
             self.cache.reserve(int(s), int(p) + 1)
         self.cache.sync_table()
-        return self._run(self._tokens(ids), self._tokens(seqs), self._tokens(positions), int(max(positions)) + 1)
+        q4, b = None, len(ids)
+        if self.cache.q4:  # every token a sequence of its own: the same one may come twice
+            rows = self.cache.table.index_select(0, self._tokens(seqs))
+            q4 = _Q4Step(self._tokens(self.cache.slots(seqs, positions)), self._tokens(range(b + 1)),
+                         self._tokens([int(p) + 1 for p in positions]), rows, 1)
+        return self._run(self._tokens(ids), self._tokens(seqs), self._tokens(positions), int(max(positions)) + 1, q4=q4)
 
     def greedy_graph(self, prompt: Sequence[int], steps: int, seq: int = 0):
         """Greedy decode of `steps` tokens after the prompt with one decode step captured as
@@ -413,8 +480,15 @@ class Qwen2Model:
         seq_d = torch.tensor([seq], dtype=torch.int32, device=self.device)
         out = torch.empty((steps,), dtype=torch.int32, device=self.device)
 
+        one = torch.tensor([0, 1], dtype=torch.int32, device=self.device)
+        row = self.cache.table[seq:seq + 1]
+
         def step():
-            self._run(tok, seq_d, pos, total, head_ids=tok)
+            q4 = None
+            if self.cache.q4:
+                slot = row[0].index_select(0, pos // KV_BLOCK) * KV_BLOCK + pos % KV_BLOCK
+                q4 = _Q4Step(slot, one, pos + 1, row, 1)
+            self._run(tok, seq_d, pos, total, head_ids=tok, q4=q4)
             pos.add_(1)
 
         # one eager step first (kernel attributes are configured outside capture); the
@@ -435,6 +509,81 @@ class Qwen2Model:
             state["i"] += 1
 
         return out, g, replay
+
+    def generate_batch(self, prompts: Sequence[Sequence[int]], steps: int, temperature: float = 1.0, top_k: int = 0,
+                       top_p: float = 1.0, min_p: float = 0.0, seed: int = 0, graph: bool = True) -> torch.Tensor:
+        """Sample `steps` tokens after each prompt (sequences 0, 1, ...): int32 ids
+        [len(prompts), steps] on the device.
+
+        A step never waits for the host: rtd_kv_plan grows the sequences by a token (their
+        blocks from the device's free stack), the layers run over the tokens it lists, and
+        rtd_sample puts the next ids where the next step reads them; with `graph` the step
+        is captured once and replayed.  The random numbers come from torch's generator
+        seeded with `seed`, one per sequence and step, so equal calls give equal ids."""
+        from . import kv4, sampling
+
+        b, cache = len(prompts), self.cache
+        if not 0 < b <= cache.max_seqs or steps < 1 or not all(len(p) for p in prompts):
+            raise ConfigError(f"{b} prompts for {cache.max_seqs} sequences, {steps} steps (a prompt has a token at least)")
+        longest = max(len(p) for p in prompts) + steps
+        for s in range(b):
+            cache.release(s)
+        need = sum(-(-(len(p) + steps) // KV_BLOCK) for p in prompts)
+        if -(-longest // KV_BLOCK) > cache.max_blocks or need > len(cache._free):
+            raise ConfigError(f"KV cache: {need} blocks for {longest} tokens of a sequence, {len(cache._free)} free, "
+                              f"{cache.max_blocks} a sequence")
+        dev, f32 = self.device, torch.float32
+        gen = torch.Generator(device=dev)
+        gen.manual_seed(seed)
+        u = torch.rand((steps, b), generator=gen, dtype=f32, device=dev)
+        filters = [torch.full((b,), temperature, dtype=f32, device=dev),
+                   torch.full((b,), top_k, dtype=torch.int32, device=dev) if top_k > 0 else None,
+                   torch.full((b,), top_p, dtype=f32, device=dev) if top_p < 1 else None,
+                   torch.full((b,), min_p, dtype=f32, device=dev) if min_p > 0 else None]
+        last = torch.cat([self.forward(list(p), 0, seq=s, last_only=True) for s, p in enumerate(prompts)])
+        out = torch.empty((steps, b), dtype=torch.int32, device=dev)
+        ids, now = torch.empty((b,), dtype=torch.int32, device=dev), u[0].clone()
+        sampling.sample(last, now, *filters, out=ids)
+        out[0].copy_(ids)
+        if steps == 1:
+            return out.t().contiguous()
+        tables = kv4.BlockTables.from_cache(cache, b)
+        grow = torch.zeros((cache.max_seqs,), dtype=torch.int32, device=dev)
+        grow[:b] = 1
+
+        def step():
+            tables.step(tables.length + grow)
+            q4 = _Q4Step(tables.tok_slot, tables.q_start, tables.length, tables.table, 1) if cache.q4 else None
+            logits = self._run(ids, tables.tok_seq, tables.tok_pos, longest, q4=q4, block_table=tables.table)
+            sampling.sample(logits, now, *filters, out=ids)
+
+        replay = step
+        if graph:
+            # one eager step first (kernel attributes are configured outside capture), taken
+            # back: the first replay writes the same positions again
+            before, first = tables.length.clone(), ids.clone()
+            step()
+            tables.set_lengths(before)
+            ids.copy_(first)
+            torch.cuda.synchronize(dev)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                step()
+            replay = g.replay
+        for i in range(1, steps):
+            now.copy_(u[i])
+            replay()
+            out[i].copy_(ids)
+        tables.into(cache)
+        return out.t().contiguous()
+
+    def sample(self, logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+               top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+               min_p: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Ids drawn from the rows of `logits` with the random numbers `u` (runtimed_b200.sampling)."""
+        from . import sampling
+
+        return sampling.sample(logits, u, temperature, top_k, top_p, min_p)
 
     def argmax(self, logits: torch.Tensor) -> torch.Tensor:
         """Greedy ids of the rows of `logits` (SubstratePort::argmax, decode/sample.rs:11-18)."""
