@@ -24,7 +24,7 @@ LIB = os.path.join(HERE, "libruntimed_b200.so")
 TORCH_LIB = os.path.join(HERE, "_rtd_torch.so")
 INCLUDE = os.path.join(ROOT, "include")
 
-SOURCES = ["rtd_api.cu", "rtd_gemv.cu", "rtd_gemm.cu", "rtd_gemm_ts.cu", "rtd_tp.cu", "rtd_model.cu", "rtd_kv4.cu",
+SOURCES = ["rtd_api.cu", "rtd_gemv.cu", "rtd_gemm.cu", "rtd_gemm_ts.cu", "rtd_tp.cu", "rtd_model.cu", "rtd_kv4.cu", "rtd_kv4_wide.cu",
            "rtd_sample.cu", "rtd_dequant.cu", "rtd_repack.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

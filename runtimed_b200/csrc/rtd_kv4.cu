@@ -1,25 +1,6 @@
 // rtd_kv4.cu -- the paged KV cache held in 4 bits, sm_100a: block tables built on the
-// device, the quantising append, the attention that reads it and a plain reader.
-//
-// A page is 16 tokens of one kv head, 20 * D bytes (D = head_dim, NG = D / 32 groups):
-//   [0, 8D)     K codes, D / 2 bytes a token     [8D, 10D)   K headers, 4 bytes a group
-//   [10D, 18D)  V codes                          [18D, 20D)  V headers
-// A header is (f16 step d, f16 minimum m); a code c stands for d * c + m, with
-// d = f16((max - min) / 15), m = f16(min) over the 32 dims of the group.  A group with a
-// value that is not finite, or whose header overflows f16, is held as d = m = NaN: reading
-// it gives NaN, as a 16-bit cache would.
-//
-// The codes lie in the order the attention's fragments want them:
-//   K: word i * NG + g of a token holds dims 32 g + 8 i .. + 7 (i < 4): lane i of a quad
-//      reads its words of every group with one load, and a warp's eight tokens are one
-//      contiguous, conflict-free span.
-//   V: word n holds, in its low and high half, dims 4 n .. 4 n + 3 of two neighbouring
-//      groups (n < 8), so that the halves of two tokens' words join into f16 pairs of one
-//      dim.  With four groups both pairs' words alternate (one 64-bit load), and tokens
-//      with bit 1 set have the words 8 apart exchanged, which spreads a quad's four tokens
-//      over all 32 banks.  A last odd group fills half words.
-// A token owns whole bytes everywhere, so tokens of one page may be appended by different
-// CTAs of one launch.
+// device, the quantising append, the attention that reads it and a plain reader.  The pages'
+// layout stands in rtd_kv4.cuh; prompt chunks with 16-bit outputs run in rtd_kv4_wide.cu.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,40 +9,11 @@
 #include <atomic>
 #include <cstdint>
 
-#include "rtd_common.cuh"
-#include "rtd_kernels.h"
+#include "rtd_kv4.cuh"
 
 namespace rtd {
 namespace {
 
-constexpr int kTok = 16;  // tokens of a page
-
-// The kernel's shared-memory limit, set once per device (a bit each in `configured`).
-template <typename K>
-cudaError_t configure_once(K kernel, int smem, std::atomic<uint64_t>& configured) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (e != cudaSuccess || (configured.load(std::memory_order_relaxed) & bit)) return e;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) configured.fetch_or(bit, std::memory_order_relaxed);
-  return e;
-}
-
-__device__ __forceinline__ float load_as_f32(const void* p, int dt, int64_t i) {
-  if (dt == 0) return static_cast<const float*>(p)[i];
-  if (dt == 1) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-
-__device__ __forceinline__ void store_from_f32(void* p, int dt, int64_t i, float v) {
-  if (dt == 0)
-    static_cast<float*>(p)[i] = v;
-  else if (dt == 1)
-    static_cast<__half*>(p)[i] = __float2half_rn(v);
-  else
-    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-}
 
 // Byte of the half word with dims 32 g + 4 n .. + 3 of V, within the token's row.
 template <int NG>
@@ -424,38 +376,9 @@ constexpr int kStages = 5;
 constexpr int kRows = 8;
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 512;
+// Sequences with so many rows (queries x heads of the group) run in the wide kernel.
+constexpr int kWideRows = 96;
 constexpr int kUnitCost = 8;  // what a unit costs beside its pages (queries, joins), in pages
-
-struct Kv4AttnArgs {
-  const void* q;
-  int q_dtype;
-  int q_wide;  // f32 rows on 16-byte boundaries
-  int64_t ldq;
-  int T, n_head, n_kv;
-  float scale;
-  const int* q_start;
-  const int* ctx_len;
-  int S;
-  const int* table;
-  int max_blocks, max_q, max_ctx;
-  const uint8_t* pages;
-  int num_blocks;
-  void* o;
-  int o_dtype;
-  int o_wide;       // f32 rows on 16-byte boundaries
-  int64_t ldo;
-  int min_share;    // pages a CTA takes at least
-  float* part;      // [CTA][2][8 (D + 2)]: the units begun before it, and left open by it
-  unsigned* count;  // [CTA]: parts done of the unit it leaves open, zero between calls
-  int* status;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // |e| <= 126
 
 __device__ __forceinline__ uint64_t f2(float a, float b) {
   uint64_t r;
@@ -477,9 +400,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ __half2 as_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
 // Nibbles 0 and 4 (ODD = false) or 1 and 5 of w as an f16 pair, odd ones times 16: c - S
 // when EXACT, else the subnormals c * 2^-24.
 template <bool EXACT, int S, bool ODD>
@@ -573,7 +493,7 @@ struct Attn {
     nq = __ldg(a.q_start + s + 1) - qs;
     ctx = __ldg(a.ctx_len + s);
     bool bad = qs < 0 || nq < 0 || (int64_t)qs + nq > a.T || nq > a.max_q;
-    if (bad) nq = 0;
+    if (bad || nq * G >= a.wide_rows) nq = 0;
     if (ctx > a.max_ctx) {
       bad |= nq > 0;
       ctx = 0;
@@ -1203,11 +1123,17 @@ cudaError_t launch_kv4_read(const int* slots, int64_t n, int n_kv, int head_dim,
 
 cudaError_t launch_kv4_attention(const Kv4Attention& c) {
   const int wide = c.q_dtype == 0 && c.ldq % 4 == 0 && reinterpret_cast<uintptr_t>(c.q) % 16 == 0;
-  const int wide_o = c.o_dtype == 0 && c.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(c.o) % 16 == 0;
+  const int wide_o = c.ldo % (c.o_dtype == 0 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(c.o) % 16 == 0;
   Kv4AttnArgs a{c.q, c.q_dtype, wide, c.ldq, (int)c.T, c.n_head, c.n_kv, c.scale, c.q_start, c.ctx_len, c.S, c.block_table,
                 c.max_blocks, c.max_q, c.max_ctx, c.pages, c.num_blocks, c.o, c.o_dtype, wide_o,
-                c.ldo,                kUnitCost + std::min(32, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
+                c.ldo, INT32_MAX, kUnitCost + std::min(32, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
   const bool exact = c.o_dtype == 0;
+  const int64_t rows = (int64_t)c.max_q * (c.n_head / c.n_kv);
+  if (!exact && (c.head_dim == 64 || c.head_dim == 128) && rows >= kWideRows) {
+    a.wide_rows = kWideRows;
+    cudaError_t e = launch_kv4_wide(a, c.head_dim, c.stream);
+    if (e != cudaSuccess) return e;  // what follows is for the others, if any
+  }
   switch (c.head_dim / 32) {
     case 1: return exact ? attn_launch<1, true>(a, c.sm_count, c.stream) : attn_launch<1, false>(a, c.sm_count, c.stream);
     case 2: return exact ? attn_launch<2, true>(a, c.sm_count, c.stream) : attn_launch<2, false>(a, c.sm_count, c.stream);
