@@ -2,23 +2,27 @@
 // against the same keys, on the tcgen05 tensor cores.
 //
 // A CTA takes (sequence, kv head, 256 rows; row = token * G + head of the group) as two
-// tiles of 128 rows, and walks the keys in tiles of 128:
+// tiles of 128 rows, and walks the keys in tiles of 64:
 //   loader      bulk copies of raw pages, two a stage, in page-table order;
-//   4 warps     turn the codes into f16 tiles d * c + m in shared memory, once for both row
+//   8 warps     turn the codes into f16 tiles d * c + m in shared memory, once for both row
 //               tiles: K [key][dim] and V transposed [dim][key], both K-major in 128-byte
-//               swizzled atoms, two buffers each;
-//   MMA thread  S = Q K^T (Q, K in shared memory) and O += P V (P in tensor memory);
+//               swizzled atoms, four buffers each;
+//   MMA thread  S = Q K^T and O += P V, Q and P in tensor memory: with Q in shared memory an
+//               MMA took 109 clocks for 64 of work, since both operands and the decoding
+//               shared its bandwidth;
 //   2 x 4 warps softmax, a thread a row, one row tile each: S from tensor memory, P back over
 //               the same columns in f16.  While one tile's softmax runs, the tensor cores
 //               work on the other's.
-// Tensor memory: S0 S1 O0 O1, 128 columns each.
+// Tensor memory: S0 S1 (64 columns each), Q0 Q1 (D / 2), O0 O1 (D).
 //
-// The running maximum moves only when a score passes it by 2^12, so O is rescaled rarely;
-// 2^(x - max + 8) stays inside f16, whose 11 bits P, K, V and the queries (scaled by a power
-// of two per row) are rounded to.  Values beyond f16's 65504 become infinite.
+// The running maximum moves only when a row's sum of p = 2^(x - max) over a key tile passes
+// 2^15: until then every p is below that, and inside f16.  So the maximum is looked for, and O
+// rescaled, rarely, and the exponentials come straight from the scores.  P, K, V and the
+// queries (scaled by a power of two per row) are rounded to f16's 11 bits; values beyond its
+// 65504 become infinite.
 //
-// Bound: per 128 x 128 scores 1024 clocks of tensor cores (at head_dim 128) and as many of
-// the exponential unit; two row tiles share the decoding, 2000 warp instructions a key tile.
+// Bound: per 128 x 64 scores 512 clocks of tensor cores (at head_dim 128) and as many of the
+// exponential unit; what they take is the chain S -> softmax -> P -> S of a row tile.
 #include <algorithm>
 #include <cstdint>
 
@@ -28,35 +32,39 @@
 namespace rtd {
 namespace {
 
-constexpr int kKeys = 128;             // keys of a tile
+constexpr int kKeys = 64;              // keys of a tile
+constexpr int kBuf = 4;                // buffers of K and V tiles
 constexpr int kStageKeys = 2 * kTok;   // keys of a raw stage
-constexpr int kRaw = 6;                // raw stages
-constexpr int kSoftWarps = 8, kDecodeWarps = 4;
+constexpr int kRaw = 12;               // raw stages
+constexpr int kSoftWarps = 8, kDecodeWarps = 8;
 constexpr int kMmaWarp = kSoftWarps + kDecodeWarps, kLoadWarp = kMmaWarp + 1;
-constexpr int kWideThreads = 512;  // and two idle warps, for a whole number of warpgroups
-// Registers: launched with 128 a thread, 65536 in all; 256 x 176 + 128 x 96 + 128 x 64 are the same.
-constexpr int kSoftRegs = 176, kDecodeRegs = 96, kOtherRegs = 64;
+constexpr int kWideThreads = 640;  // and two idle warps, for a whole number of warpgroups
+// Registers: launched with 96 a thread, 61440 in all; 256 x 128 + 256 x 80 + 128 x 64 are the same.
+constexpr int kSoftRegs = 128, kDecodeRegs = 80, kOtherRegs = 64;
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-constexpr float kHeadroom = 8.0f, kGrowth = 12.0f;
+constexpr float kHeadroom = 8.0f, kMostSum = 32768.0f;  // 64 times 2^8 is below it
 
 template <int NG>
 struct WidePlan {
   static constexpr int D = 32 * NG, PB = 20 * D;
-  static constexpr int kTile = kKeys * D * 2;  // a K or V tile, or 128 queries
-  static constexpr int offQ = 0;
-  static constexpr int offK = offQ + 2 * kTile;
-  static constexpr int offV = offK + 2 * kTile;
-  static constexpr int offRaw = offV + 2 * kTile;
+  static constexpr int kTile = kKeys * D * 2;  // a K or V tile
+  static constexpr int offK = 0;
+  static constexpr int offV = offK + kBuf * kTile;
+  static constexpr int offRaw = offV + kBuf * kTile;
+  static constexpr int offQ = 0;               // the queries on their way to tensor memory: before any K and V
+  static constexpr int kQTile = 128 * D * 2;
+  static_assert(2 * kQTile <= offRaw, "the queries lie where K and V will");
+  static constexpr uint32_t colS = 0, colQ = 2 * kKeys, colO = colQ + D;  // tensor-memory columns
   static constexpr int offBar = offRaw + kRaw * 2 * PB;
   static constexpr int kSmem = offBar + 512 + 1024;  // and the alignment of the tiles
 };
 
-// 32 accumulator columns of this warp's lanes.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 columns of this warp's lanes, to be waited for with tmem_wait_ld: the registers pass
+// through the wait, so that no use is scheduled before it.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
       "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -65,17 +73,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
-  // the registers pass through the wait, so that no use is scheduled before it
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27])
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14])
                :
                : "memory");
-  asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+  asm volatile("" : "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                    "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]));
+  asm volatile("" : "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
   asm volatile(
@@ -88,11 +95,47 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
       : "memory");
 }
 
+// D (+)= A[tmem] . B[smem desc]^T, f16 in, f32 out.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+
 // Nibbles 0 and 4 (ODD = false) or 1 and 5 of w as the f16 pair c, exactly.
 template <bool ODD>
 __device__ __forceinline__ __half2 code_pair(uint32_t w) {
   const __half2 h = as_h2(lop_and_or(w, ODD ? 0x00F000F0u : 0x000F000Fu, 0x64006400u));
   return ODD ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-64.0f)) : __hadd2(h, __float2half2_rn(-1024.0f));
+}
+
+__device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
 }
 
 template <int NG>
@@ -104,9 +147,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
   const uint32_t sm32 = smem_u32(sm);
   uint64_t* raw_full = reinterpret_cast<uint64_t*>(sm + P::offBar);
   uint64_t* raw_empty = raw_full + kRaw;
-  uint64_t* kv_full = raw_empty + kRaw;   // [2]
-  uint64_t* kv_empty = kv_full + 2;       // [2]
-  uint64_t* s_full = kv_empty + 2;        // [row tile]: S is there, and O of the key tile before
+  uint64_t* kv_full = raw_empty + kRaw;   // [kBuf]
+  uint64_t* kv_empty = kv_full + kBuf;    // [kBuf]
+  uint64_t* s_full = kv_empty + kBuf;     // [row tile]: S is there, and O of the key tile before
   uint64_t* p_full = s_full + 2;          // [row tile]
   uint64_t* q_full = p_full + 2;
   uint64_t* drained = q_full + 1;
@@ -132,7 +175,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
   const int nraw = (pages + 1) / 2;                       // raw stages
   const int qtiles = rows - row0 > 128 ? 2 : 1;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(misc), 512);
     tmem_relinquish();
@@ -140,11 +183,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
   if (tid == 0) {
     for (int i = 0; i < kRaw; ++i) {
       mbar_init(raw_full + i, 1);
-      mbar_init(raw_empty + i, 32 * kDecodeWarps);
+      mbar_init(raw_empty + i, 16 * kDecodeWarps);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kBuf; ++i) {
       mbar_init(kv_full + i, 32 * kDecodeWarps);
       mbar_init(kv_empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
     }
@@ -212,51 +257,56 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
       for (int k = max(0, i - kRaw); k < i; ++k) mbar_wait_ns(raw_full + k % kRaw, (uint32_t)((k / kRaw) & 1), kWaitBudgetNs, a.status);
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA
-    if (lane == 0 && nt > 0) {
+    // The whole warp walks the loop and one elected lane issues, so that descriptors stay in
+    // uniform registers: issued from a one-lane branch an MMA took 118 clocks.
+    if (nt > 0) {
       const uint32_t idesc_s = idesc_f16(kKeys), idesc_o = idesc_f16(D);
+      const uint64_t k0 = kmajor_desc(sm32 + P::offK), v0 = kmajor_desc(sm32 + P::offV);
+      const bool issuer = elect_one();
       auto scores = [&](int t, int buf) {
+        const uint64_t b = k0 + (uint64_t)(buf * (P::kTile >> 4));
+        const uint32_t d = tmem + P::colS + kKeys * t, q = tmem + P::colQ + (D / 2) * t;
+        if (issuer) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (uint32_t)((k / 4) * (128 * 128) + (k % 4) * 32);
-          umma_f16(tmem + 128u * t, kmajor_desc(sm32 + P::offQ + t * P::kTile + off),
-                   kmajor_desc(sm32 + P::offK + buf * P::kTile + off), idesc_s, k > 0);
+          for (int k = 0; k < D / 16; ++k)
+            umma_ts(d, q + 8u * k, b + (uint64_t)((k / 4) * (kKeys * 8) + (k % 4) * 2), idesc_s, k > 0);
+          umma_commit(s_full + t);
         }
       };
       auto output = [&](int t, int buf, bool more) {
+        const uint64_t b = v0 + (uint64_t)(buf * (P::kTile >> 4));
+        const uint32_t d = tmem + P::colO + D * t, p = tmem + P::colS + kKeys * t;
+        if (issuer) {
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k) {
-          const uint32_t off = (uint32_t)((k / 4) * (D * 128) + (k % 4) * 32);
-          umma_f16_ts(tmem + 256u + 128u * t, tmem + 128u * t + 8u * k, kmajor_desc(sm32 + P::offV + buf * P::kTile + off), idesc_o,
-                      more || k > 0);
+          for (int k = 0; k < kKeys / 16; ++k) umma_ts(d, p + 8u * k, b + (uint64_t)(2 * k), idesc_o, more || k > 0);
         }
       };
       bool ok = wait(q_full, 0) && wait(kv_full, 0);
+      ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
-        for (int t = 0; t < qtiles; ++t) {
-          scores(t, 0);
-          umma_commit(s_full + t);
-        }
+        for (int t = 0; t < qtiles; ++t) scores(t, 0);
         for (int j = 0; j < nt && ok; ++j) {
           for (int t = 0; t < qtiles && ok; ++t) {
             ok = wait(p_full + t, (uint32_t)(j & 1));
+            if (t == 0 && j + 1 < nt && ok) ok = wait(kv_full + (j + 1) % kBuf, (uint32_t)(((j + 1) / kBuf) & 1));
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            output(t, j & 1, j > 0);
-            if (t == qtiles - 1) umma_commit(kv_empty + (j & 1));  // both tiles are done with these keys
-            if (j + 1 < nt) {
-              if (t == 0) ok = wait(kv_full + ((j + 1) & 1), (uint32_t)(((j + 1) >> 1) & 1));
-              if (!ok) break;
-              tc_fence_after();
-              scores(t, (j + 1) & 1);  // over P, whose product was issued before
-            }
-            umma_commit(s_full + t);
+            output(t, j % kBuf, j > 0);
+            if (issuer && t == qtiles - 1) umma_commit(kv_empty + j % kBuf);  // both tiles are done with these keys
+            if (j + 1 < nt)
+              scores(t, (j + 1) % kBuf);  // over P, whose product was issued before
+            else if (issuer)
+              umma_commit(s_full + t);  // O is there
           }
         }
       }
       // an aborted run leaves MMAs in flight
-      umma_commit(drained);
-      mbar_wait_ns(drained, 0, kWaitBudgetNs, a.status);
+      if (issuer) {
+        umma_commit(drained);
+        mbar_wait_ns(drained, 0, kWaitBudgetNs, a.status);
+      }
     }
     __syncwarp();
   } else if (warp >= kMmaWarp) {
@@ -264,17 +314,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
   } else if (warp >= kSoftWarps) {
     // ------------------------------------------------------------ decode
     regs_down<kDecodeRegs>();
-    const int dt = tid - 32 * kSoftWarps, dw = dt >> 5;
-    bool ok = true;
-    // K: (token, quarter of 8 dims in every group); tokens t and t + 4 share eight lanes, whose
-    // stores then fill all banks
-    const int kt = 8 * dw + ((lane >> 3) & 3) + 4 * ((lane >> 2) & 1), ki = lane & 3;
-    // V: (eight keys, four dims of a group): octets and the parity of n in the low bits, likewise
-    const int oct = lane & 3, vn = ((lane >> 2) & 1) | (lane >> 3) << 1, vg = dw;
+    // Four warps take the even stages, four the odd ones; of four, two turn K and two V.
+    const int dw = (warp - kSoftWarps) & 3, odd_stage = (warp - kSoftWarps) >> 2;
+    bool ok = nt == 0 || wait(q_full, 0);  // the queries have left
     for (int j = 0; j < nt && ok; ++j) {
-      const int buf = j & 1;
-      if (j >= 2) ok = wait(kv_empty + buf, (uint32_t)(((j >> 1) - 1) & 1));
-      for (int q = 0; q < kKeys / kStageKeys && ok; ++q) {
+      const int buf = j % kBuf;
+      if (j >= kBuf) ok = wait(kv_empty + buf, (uint32_t)((j / kBuf - 1) & 1));
+      for (int q = odd_stage; q < kKeys / kStageKeys && ok; q += 2) {
         const int i = j * (kKeys / kStageKeys) + q, st = i % kRaw;
         const uint32_t raw = sm32 + P::offRaw + st * 2 * PB;
         const int key = i * kStageKeys;
@@ -282,76 +328,107 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
           ok = wait(raw_full + st, (uint32_t)((i / kRaw) & 1));
           if (!ok) break;
         }
-        {  // K, [key][dim]; a quarter's dims in the order 0 4 1 5 2 6 3 7, as the queries'
-          const int t = kt & 15;
-          const uint32_t page = raw + (kt >> 4) * PB;
-          const bool there = key + kt < most;
-          const int row = q * kStageKeys + kt;
-          // A NaN of V that some rows of the tile do not see would reach them as 0 * NaN.  From
-          // the first row's position on it goes into the key instead, whose score only the
-          // rows that see it take.
-          bool poison = false;
-          if (key + kStageKeys > least && there && key + kt >= least) {
+        if (dw < 2) {
+          // K, [key][dim]: a thread has a quarter (8 dims) of every group of two tokens; the
+          // dims in the order 0 4 1 5 2 6 3 7, as the queries'.  Tokens t and t + 4 share
+          // eight lanes, whose stores then fill all banks.
+          const int ki = lane & 3;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) poison |= (lds32(page + 18 * D + (t * NG + g) * 4) & 0x7c00u) == 0x7c00u;
-          }
+          for (int half = 0; half < 2; ++half) {
+            const int kt = 16 * dw + 8 * half + ((lane >> 3) & 3) + 4 * ((lane >> 2) & 1), t = kt & 15;
+            const uint32_t page = raw + (kt >> 4) * PB;
+            const bool there = key + kt < most;
+            const int row = q * kStageKeys + kt;
+            // A NaN of V that some rows of the tile do not see would reach them as 0 * NaN.  From
+            // the first row's position on it goes into the key instead, whose score only the
+            // rows that see it take.
+            bool poison = false;
+            if (key + kStageKeys > least && there && key + kt >= least) {
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            __half2 v[4] = {};
-            if (there) {
-              const uint32_t w = lds32(page + t * (D / 2) + (ki * NG + g) * 4), h = lds32(page + 8 * D + (t * NG + g) * 4);
-              const __half2 d = __low2half2(as_h2(h)), m = __high2half2(as_h2(h));
-              v[0] = __hfma2(code_pair<false>(w), d, m);
-              v[1] = __hfma2(code_pair<true>(w), d, m);
-              v[2] = __hfma2(code_pair<false>(w >> 8), d, m);
-              v[3] = __hfma2(code_pair<true>(w >> 8), d, m);
-              if (poison) v[0] = as_h2(0x7fff7fffu);
+              for (int g = 0; g < NG; ++g) poison |= (lds32(page + 18 * D + (t * NG + g) * 4) & 0x7c00u) == 0x7c00u;
             }
-            const int k = 32 * g + 8 * ki;
-            sts128(sm32 + P::offK + buf * P::kTile + (k >> 6) * (128 * 128) + sw_off(row, k & 63), as_u32(v[0]), as_u32(v[1]),
-                   as_u32(v[2]), as_u32(v[3]));
+            uint32_t w[4] = {}, h[4] = {};
+            if (there) {
+              const uint32_t at = page + t * (D / 2) + ki * NG * 4, head = page + 8 * D + t * NG * 4;
+              if constexpr (NG == 4) {
+                *reinterpret_cast<uint4*>(w) = lds128(at);
+                *reinterpret_cast<uint4*>(h) = lds128(head);
+              } else {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                  w[g] = lds32(at + 4 * g);
+                  h[g] = lds32(head + 4 * g);
+                }
+              }
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              const __half2 d = __low2half2(as_h2(h[g])), m = __high2half2(as_h2(h[g]));
+              uint32_t v0 = as_u32(__hfma2(code_pair<false>(w[g]), d, m));
+              if (poison) v0 = 0x7fff7fffu;
+              const int k = 32 * g + 8 * ki;
+              sts128(sm32 + P::offK + buf * P::kTile + (k >> 6) * (kKeys * 128) + sw_off(row, k & 63), v0,
+                     as_u32(__hfma2(code_pair<true>(w[g]), d, m)), as_u32(__hfma2(code_pair<false>(w[g] >> 8), d, m)),
+                     as_u32(__hfma2(code_pair<true>(w[g] >> 8), d, m)));
+            }
           }
-        }
-        if (vg < NG) {  // V, [dim][key]
+        } else if (2 * (dw - 2) < NG) {
+          // V, [dim][key]: a thread has eight keys (an octet) of four dims in each of two
+          // groups.  Octets and the parity of n lie in the low lane bits, so that eight lanes'
+          // stores fill all banks; odd octets read the tokens of a pair in turn.
+          const int oct = lane & 3, n = ((lane >> 2) & 1) | (lane >> 3) << 1, gp = dw - 2, swap = oct & 1;
           const uint32_t page = raw + (oct >> 1) * PB + 10 * D;
+          const uint32_t low = swap ? 0x1054u : 0x5410u, high = swap ? 0x3276u : 0x7632u;
           const int t0 = 8 * (oct & 1);
-          uint32_t w[8], h[8];
+          // every load before the first store: the compiler cannot tell them apart
+          uint32_t w[8], h[8][2];
+          const bool whole = key + kStageKeys <= most;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int t = t0 + e;
+            const int t = t0 + (e ^ swap);
             uint32_t at;
             if constexpr (NG == 4)
-              at = (uint32_t)((((vn * 2 + (vg >> 1)) ^ (8 * ((t >> 1) & 1))) << 2) + (vg & 1) * 2);
+              at = (uint32_t)(((n * 2 + gp) ^ (8 * ((t >> 1) & 1))) << 2);
             else
-              at = (uint32_t)(vn * 4 + (vg & 1) * 2);
-            const bool there = key + 8 * oct + e < most;
-            w[e] = there ? lds16(page + t * (D / 2) + at) : 0;
-            h[e] = there ? lds32(page + 8 * D + (t * NG + vg) * 4) : 0;
+              at = (uint32_t)(n * 4);
+            w[e] = lds32(page + t * (D / 2) + at);
+            const uint2 hh = lds64(page + 8 * D + (t * NG + 2 * gp) * 4);
+            h[e][0] = hh.x;
+            h[e][1] = hh.y;
           }
-          uint32_t out[4][4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t x = w[2 * e] | (w[2 * e + 1] << 16);
-            const __half2 d = as_h2(prmt(h[2 * e], h[2 * e + 1], 0x5410u)), m = as_h2(prmt(h[2 * e], h[2 * e + 1], 0x7632u));
-            out[0][e] = as_u32(__hfma2(code_pair<false>(x), d, m));
-            out[1][e] = as_u32(__hfma2(code_pair<true>(x), d, m));
-            out[2][e] = as_u32(__hfma2(code_pair<false>(x >> 8), d, m));
-            out[3][e] = as_u32(__hfma2(code_pair<true>(x >> 8), d, m));
-          }
-          if (key + kStageKeys > least) {
+          if (!whole) {  // past the last key, and what was never loaded
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (key + 8 * oct + e >= least && (h[e] & 0x7c00u) == 0x7c00u) {
-#pragma unroll
-                for (int p = 0; p < 4; ++p) out[p][e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
-              }
+              if (key + 16 * (oct >> 1) + t0 + (e ^ swap) >= most) w[e] = h[e][0] = h[e][1] = 0;
           }
+          const bool diag = key + kStageKeys > least;
           const int k = q * kStageKeys + 8 * oct;
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            const int d = 32 * vg + 4 * vn + p;
-            sts128(sm32 + P::offV + buf * P::kTile + (k >> 6) * (D * 128) + sw_off(d, k & 63), out[p][0], out[p][1], out[p][2],
-                   out[p][3]);
+          for (int g = 0; g < 2; ++g) {
+            uint32_t out[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = prmt(w[2 * e], w[2 * e + 1], g ? high : low);
+              const __half2 d = as_h2(prmt(h[2 * e][g], h[2 * e + 1][g], low)), m = as_h2(prmt(h[2 * e][g], h[2 * e + 1][g], high));
+              out[0][e] = as_u32(__hfma2(code_pair<false>(x), d, m));
+              out[1][e] = as_u32(__hfma2(code_pair<true>(x), d, m));
+              out[2][e] = as_u32(__hfma2(code_pair<false>(x >> 8), d, m));
+              out[3][e] = as_u32(__hfma2(code_pair<true>(x >> 8), d, m));
+              if (diag) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                  const int tok = b ^ swap;  // the half it lies in
+                  if (key + 16 * (oct >> 1) + t0 + 2 * e + tok >= least && (h[2 * e + b][g] & 0x7c00u) == 0x7c00u) {
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) out[p][e] &= tok ? 0x0000ffffu : 0xffff0000u;
+                  }
+                }
+              }
+            }
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+              sts128(sm32 + P::offV + buf * P::kTile + sw_off(32 * (2 * gp + g) + 4 * n + p, k), out[p][0], out[p][1], out[p][2],
+                     out[p][3]);
           }
         }
         if (i < nraw) mbar_arrive(raw_empty + st);
@@ -364,7 +441,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
     regs_up<kSoftRegs>();
     const int t = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t ts = tmem + lanes + 128u * t, to = tmem + lanes + 256u + 128u * t;
+    const uint32_t ts = tmem + lanes + P::colS + kKeys * t, to = tmem + lanes + P::colO + D * t;
     const int row = row0 + 128 * t + r;
     const bool live = row < rows;
     const int limit = live ? seen(row) : 0;
@@ -402,9 +479,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
         const bool odd = lane & 1;
         const float y0 = __shfl_xor_sync(0xffffffffu, odd ? x[0] : x[2], 1), y1 = __shfl_xor_sync(0xffffffffu, odd ? x[1] : x[3], 1);
         const uint32_t w0 = odd ? pack_f16x2(y0, x[2]) : pack_f16x2(x[0], y0), w1 = odd ? pack_f16x2(y1, x[3]) : pack_f16x2(x[1], y1);
-        const int d8 = d0 & ~7;
-        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(sm32 + P::offQ + t * P::kTile + (d8 >> 6) * (128 * 128) +
-                                                             sw_off(wr, d8 & 63) + (odd ? 8 : 0)),
+        // 16-byte chunk c of row r at c ^ (r & 7)
+        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(sm32 + P::offQ + t * P::kQTile + wr * (2 * D) +
+                                                             (((d0 >> 3) ^ (wr & 7)) << 4) + (odd ? 8 : 0)),
                      "r"(w0), "r"(w1)
                      : "memory");
 #pragma unroll
@@ -413,7 +490,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
           if (lane == r0 + e) rowmul = rm;
         }
       }
-      fence_async_shared();
+      __syncwarp();  // the row that a thread takes is its warp's own
+#pragma unroll
+      for (int c = 0; c < D / 2; c += 32) {
+        uint32_t v[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(v + 4 * e) = lds128(sm32 + P::offQ + t * P::kQTile + r * (2 * D) + (((c / 4 + e) ^ (r & 7)) << 4));
+        tmem_st32(tmem + lanes + P::colQ + (D / 2) * t + c, v);
+      }
+      tmem_wait_st();
+      tc_fence_before();
       mbar_arrive(q_full);
 
       float M = -1e30f, l = 0.0f;
@@ -425,51 +512,63 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
         tc_fence_after();
         const int key0 = j * kKeys;
         const bool masked = __any_sync(0xffffffffu, key0 + kKeys > limit);
-        uint32_t p[64];
-        float sum, top;
-        for (;;) {
-          sum = 0.0f;
-          top = -INFINITY;
+        uint32_t p[32];
+        float sum;
+        for (int again = 0;; ++again) {
+          const float2 nm = make_float2(-M, -M), rm = make_float2(rowmul, rowmul);
+          float2 acc = make_float2(0.0f, 0.0f);
+          uint32_t x[2][32];
+          tmem_ld32(ts, x[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float x[32];
-            tmem_ld32(ts + 32u * c, x);
+          for (int c = 0; c < 2; ++c) {
+            uint32_t(&v)[32] = x[c & 1];
+            tmem_wait_ld(v);
+            if (c < 1) tmem_ld32(ts + 32u * (c + 1), x[(c + 1) & 1]);
             if (masked) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (key0 + 32 * c + e >= limit) x[e] = -INFINITY;
+                if (key0 + 32 * c + e >= limit) v[e] = 0xff800000u;  // -inf
             }
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              top = fmaxf(top, fmaxf(x[e], x[e + 1]));
-              const float p0 = ex2(fmaf(x[e], rowmul, -M)), p1 = ex2(fmaf(x[e + 1], rowmul, -M));
-              sum += p0 + p1;
-              p[16 * c + e / 2] = pack_f16x2(p0, p1);
+              const float2 y = fma_f32x2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), rm, nm);
+              const float2 z = make_float2(ex2(y.x), ex2(y.y));
+              acc = add_f32x2(acc, z);
+              p[16 * c + e / 2] = pack_f16x2(z.x, z.y);
             }
           }
-          const float at = top * rowmul;
-          const bool over = at > M + kGrowth;
-          if (!__any_sync(0xffffffffu, over)) break;
+          sum = acc.x + acc.y;
+          const bool over = sum > kMostSum;
+          if (again == 2 || !__any_sync(0xffffffffu, over)) break;  // once is enough below scores of 2^24
           // a new maximum: O and l so far in its terms, and these scores once more
-          const float to_m = over ? at - kHeadroom : M, f = ex2(M - to_m);
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t v[32];
+            tmem_ld32(ts + 32u * c, v);
+            tmem_wait_ld(v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (key0 + 32 * c + e < limit) top = fmaxf(top, __uint_as_float(v[e]));
+          }
+          const float to_m = over ? top * rowmul - kHeadroom : M, f = ex2(M - to_m);
           M = to_m;
           l *= f;
           if (j > 0) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
-              float x[32];
-              tmem_ld32(to + c, x);
-              uint32_t y[32];
+              uint32_t v[32];
+              tmem_ld32(to + c, v);
+              tmem_wait_ld(v);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(x[e] * f);
-              tmem_st32(to + c, y);
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+              tmem_st32(to + c, v);
             }
             tmem_wait_st();
           }
         }
         l += sum;
         tmem_st32(ts, p);
-        tmem_st32(ts + 32u, p + 32);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_full + t);
@@ -485,11 +584,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
       const bool none = nt == 0 || l == 0.0f;
 #pragma unroll 1
       for (int c = 0; c < D && ok; c += 32) {
+        uint32_t v[32];
         float x[32];
         __syncwarp();
-        if (nt > 0) tmem_ld32(to + c, x);
+        if (nt > 0) {
+          tmem_ld32(to + c, v);
+          tmem_wait_ld(v);
+        }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = none ? 0.0f : x[e] * f;
+        for (int e = 0; e < 32; ++e) x[e] = none ? 0.0f : __uint_as_float(v[e]) * f;
         if (!live) {
         } else if (a.o_wide) {
           uint4 q[4];
