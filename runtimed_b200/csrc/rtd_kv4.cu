@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const int* slots, int64_t
 // The products run on the tensor cores on the codes themselves, and step and minimum are
 // applied to the 32-bit sums of each group:  q.k = sum_g d_g (q_g . c_g) + m_g sum(q_g),
 // the minima's part as one more MMA over the groups.  For V the weights p * d_g multiply
-// the codes, and one MMA of p with the headers gives sum p m_g and sum p d_g.
+// the codes, and one MMA of p with the headers gives the minima's part.
 //
 // EXACT (f32 outputs): rows 0..7 of the 16-row MMA hold the f16 heads of q and p d, rows
 // 8..15 the remainders, so that both enter with 22 bits (p d is split by an exact fma).  A
@@ -370,10 +370,19 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const int* slots, int64_t
 // Otherwise (16-bit outputs): the rows enter rounded to 11 bits and the nibble stays the
 // f16 subnormal c * 2^-24, which saves the addition; the tensor cores align a subnormal's
 // product as if its leading zeros counted, which costs 2e-5 of the output.
+//
+// Bound: 64 sequences of up to 4096 tokens, 64 query heads on 8 (f32 outputs) read 240 MB,
+// 37 us at the copy rate; the kernel takes 106 us (2.3 TB/s), 3 sequences of up to 60000 in
+// bf16 (184 MB, 28 us) 74 us.  It is the instructions: a page costs a warp 480 with f32 outputs, and the
+// three warps of a scheduler issue in 60 % of the cycles.  With the scores left out the
+// kernel took 80 us, with the values 85, with both 65.  Two CTAs an SM with rings of eight
+// pages and four with rings of three were no faster, nor was a loop over page pairs; five
+// stages took 110 us with f32 outputs and 75 in bf16.
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr int kStages = 5;
+constexpr int kStages = 4;  // even: pages are asked for in pairs (six do not fit three CTAs)
 constexpr int kRows = 8;
+constexpr int kFlush = 16;  // pages a warp sums up on the tensor cores alone
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 512;
 // Sequences with so many rows (queries x heads of the group) run in the wide kernel.
@@ -477,6 +486,10 @@ struct Attn {
   unsigned get = 0, phase = 0;  // the ring's next page to use, and its parity
   unsigned put_at = 0;          // the ring's next page to ask for
 
+  // A unit that other CTAs share: CTAs c0 .. c1 hold parts of it (c0 = -1: none).
+  struct Open {
+    int qs, rows, kvh, row0, c0, c1, last;
+  };
   // A stretch of one unit: what its sequence is, and this warp's pages in it.
   struct Seg {
     int s, qs, nq, ctx, kvh, tile;
@@ -506,46 +519,52 @@ struct Attn {
   // keys that a row of the sequence sees: those before and at its position
   __device__ int seen(const Seg& g, int row) const { return max(0, g.ctx - g.nq + row / G + 1); }
 
-  __device__ void issue(Seg& g, int j) {  // ask for this warp's j-th page
+  __device__ int load_ids(const Seg& g, int j) const {  // 32 of this warp's block ids from the j-th on
+    return j + lane < g.mine ? __ldg(g.table + (j + lane) * kAttnWarps) : 0;
+  }
+  // Asks for this warp's j-th and j + 1-st pages (j even), a lane each.
+  __device__ void issue(Seg& g, int j) {
     if (j >= g.mine) return;
     if ((j & 31) == 0) {
-      g.ids = 0;
-      if (j + lane < g.mine) {
-        g.ids = __ldg(g.table + (j + lane) * kAttnWarps);
-        if ((unsigned)g.ids >= (unsigned)a.num_blocks) {
-          g.bad = true;
-          g.ids = 0;
-        }
+      if (j > 0) g.ids = load_ids(g, j);
+      if ((unsigned)g.ids >= (unsigned)a.num_blocks) {
+        g.bad = true;
+        g.ids = 0;
       }
     }
-    const int blk = __shfl_sync(0xffffffffu, g.ids, j & 31);
-    if (lane == 0) {
-      mbar_arrive_expect_tx(bars + put_at, PB);
-      bulk_g2s(ring + put_at * PB, a.pages + ((int64_t)blk * a.n_kv + g.kvh) * PB, PB, bars + put_at);
+    const int blk = __shfl_sync(0xffffffffu, g.ids, (j + lane) & 31);
+    if (lane < 2 && j + lane < g.mine) {
+      unsigned at = put_at + lane;
+      if (at >= kStages) at -= kStages;
+      mbar_arrive_expect_tx(bars + at, PB);
+      bulk_g2s(ring + at * PB, a.pages + ((int64_t)blk * a.n_kv + g.kvh) * PB, PB, bars + at);
     }
-    if (++put_at == kStages) put_at = 0;
+    put_at += min(2, g.mine - j);
+    if (put_at >= kStages) put_at -= kStages;
   }
 
-  // Sets up pages [off, off + n) of a unit's line and asks for this warp's first ones.
-  __device__ void begin(Seg& g) {
+  // This warp's pages of the stretch [off, off + n) of a unit's line, and the first block ids.
+  __device__ void open(Seg& g) const {
     const int row0 = g.tile * kRows, rows = g.nq * G;
     const int need = (seen(g, min(row0 + kRows, rows) - 1) + kTok - 1) / kTok;
     g.first = max(0, g.off - kUnitCost) + warp;
     const int last = min(g.off + g.n - kUnitCost, need);
     g.mine = last > g.first ? (last - g.first + kAttnWarps - 1) / kAttnWarps : 0;
     g.table = a.table + (int64_t)g.s * a.max_blocks + g.first;
+  }
+  __device__ void begin(Seg& g) {
     g.bad = false;
-    for (int j = 0; j < kStages; ++j) issue(g, j);
+    for (int j = 0; j < kStages; j += 2) issue(g, j);
   }
 
-  __device__ void run(Place& w) {
+  __device__ void run(Place& w, Seg* next, Open* left) {
     Seg g;
     g.s = w.s;
     g.cost = seq_info(g.s, g.qs, g.nq, g.ctx, false);
     int tiles = (g.nq * G + kRows - 1) / kRows;
     int64_t unit = w.off / g.cost;  // within the sequence: kv head * tiles + tile
     g.off = (int)(w.off - unit * g.cost);
-    auto locate = [&](Seg& g) {
+    auto locate = [&](Seg& g, int64_t pos) {
       while (unit >= (int64_t)a.n_kv * tiles) {  // on to the next sequence with queries
         unit = 0;
         ++g.s;
@@ -554,32 +573,215 @@ struct Attn {
       }
       g.kvh = (int)(unit / tiles);
       g.tile = (int)(unit - (int64_t)g.kvh * tiles);
-      g.n = (int)min((int64_t)(g.cost - g.off), w.end - w.pos);
+      g.n = (int)min((int64_t)(g.cost - g.off), w.end - pos);
     };
-    locate(g);
+    locate(g, w.pos);
+    open(g);
+    g.ids = load_ids(g, 0);
     begin(g);
+    if (threadIdx.x == 0) left[0].c0 = left[1].c0 = -1;
     for (;;) {
-      const Seg done = g;
       const int64_t at = w.pos - g.off;  // the unit's place on the line
-      float M, l, o[NG][4][4], z[4];
-      pages(g, M, l, o, z);
-      const bool bad = g.bad;
       w.pos += g.n;
       const bool more = w.pos < w.end;
-      if (more) {  // the next stretch's pages are on their way while this one's warps join
-        g.off = 0;
+      int ids = 0;
+      if (more) {
+        // the next stretch: where it lies, kept in shared memory, its first block ids and its
+        // queries on their way while this one is worked on
+        Seg n = g;
+        n.off = 0;
         ++unit;
-        locate(g);
+        locate(n, w.pos);
+        open(n);
+        ids = load_ids(n, 0);
+        const int row = n.tile * kRows + (lane >> 2), es = a.q_dtype == 0 ? 4 : 2;
+        if (row < n.nq * G && (lane & 3) * 128 < D * es) {
+          const char* q = static_cast<const char*>(a.q) +
+                          ((int64_t)(n.qs + row / G) * a.ldq + (int64_t)(n.kvh * G + row % G) * D) * es + (lane & 3) * 128;
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+        }
+        if (lane == 0) *next = n;
+      }
+      float M, l, o[NG][4][4], z[4];
+      bool held;
+      pages(g, M, l, o, z, held);
+      const Seg done = g;
+      if (more) {
+        __syncwarp();
+        g = *next;
+        g.ids = ids;
         begin(g);
       }
-      finish(w, done, at, bad, M, l, o, z);
+      finish(w, done, at, M, l, o, z, held, left);
       if (!more) break;
+    }
+    join_parts(left);
+  }
+
+  // Scores of tokens 8 u + i and 8 u + 4 + i of a page (quad lane i), in the row's scale.
+  __device__ uint64_t scores(uint32_t page, int u, int kt, int qi, const uint32_t (&qm)[3]) const {
+    uint32_t kw[NG], h0[NG], h1[NG], hm[2] = {0, 0};
+    const uint32_t ph = page + 8 * D + 8 * u * (4 * NG);
+    lds_row<NG>(page + (8 * u + kt) * (D / 2) + qi * (4 * NG), kw);
+    lds_row<NG>(ph + qi * (4 * NG), h0);
+    lds_row<NG>(ph + (4 + qi) * (4 * NG), h1);
+    if constexpr (NG == 4) {
+      lds(ph + kt * 16 + 8 * (qi & 1), hm);
+    } else {
+      if (2 * qi < NG) hm[0] = lds(ph + kt * (4 * NG) + 8 * qi);
+      if (2 * qi + 1 < NG) hm[1] = lds(ph + kt * (4 * NG) + 8 * qi + 4);
+    }
+    float acc[4];
+    uint32_t bm = prmt(hm[0], hm[1], 0x7632u);
+    if (qi >= 2) bm = 0;
+    mma0(acc, qm[0], EXACT ? qm[1] : 0u, EXACT ? qm[2] : 0u, 0u, bm, EXACT ? bm : 0u);
+    uint64_t x2 = EXACT ? add2(f2(acc[0], acc[1]), f2(acc[2], acc[3])) : f2(acc[0], acc[1]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t hw = kw[g] >> 8;
+      float e[4];
+      uint32_t qa[4];
+      lds(qfrag + g * 1024, qa);
+      mma0(e, qa[0], EXACT ? qa[1] : 0u, qa[2], EXACT ? qa[3] : 0u, codes<EXACT, 0, false>(kw[g]), codes<EXACT, 0, true>(kw[g]));
+      lds(qfrag + g * 1024 + 512, qa);
+      mma(e, qa[0], EXACT ? qa[1] : 0u, qa[2], EXACT ? qa[3] : 0u, codes<EXACT, 0, false>(hw), codes<EXACT, 0, true>(hw));
+      float d0 = __low2float(as_h2(h0[g])), d1 = __low2float(as_h2(h1[g]));
+      uint64_t sum = f2(e[0], e[1]);
+      if constexpr (EXACT) {
+        sum = add2(sum, f2(e[2], e[3]));
+      } else {
+        d0 *= 16777216.0f;  // the codes' 2^-24
+        d1 *= 16777216.0f;
+      }
+      x2 = fma2(f2(d0, d1), sum, x2);
+    }
+    return x2;
+  }
+
+  // O += (p d) C and the header sums z of a page, p = ph + pl of pairs of tokens (i, i + 4) and
+  // (i + 8, i + 12).
+  __device__ void values(uint32_t page, int attempt, int r, int qi, const uint32_t (&ph)[2], const uint32_t (&pl)[2],
+                         float (&o)[NG][4][4], float (&z)[4]) const {
+    // ---- sums of p times what a group's codes add to: its minimum, or, about code 8, the
+    // middle m + 8 d.  The middles lie around zero, where the sums of the minima and of the
+    // steps would each grow and then cancel; column g takes the middle as f16, column 4 + g
+    // the rest (two-sum).  On a second attempt, whose 8 d may pass f16's range, an eighth.
+    const uint32_t vh = page + 18 * D;
+    {
+      const int g = min(r & 3, NG - 1);
+      const uint32_t at = vh + 4 * (qi * NG + g);
+      uint32_t b[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t w0 = lds(at + 32 * NG * u), w1 = lds(at + 32 * NG * u + 16 * NG);
+        b[u] = prmt(w0, w1, 0x7632u);
+        if constexpr (EXACT) {
+          const __half2 s8 = __float2half2_rn(attempt ? 1.0f : 8.0f), s1 = __float2half2_rn(attempt ? 0.125f : 1.0f);
+          const __half2 x = __hmul2_rn(as_h2(prmt(w0, w1, 0x5410u)), s8), y = __hmul2_rn(as_h2(b[u]), s1);
+          const __half2 sum = __hadd2_rn(x, y), v = __hsub2_rn(sum, x);
+          const __half2 rest = __hadd2_rn(__hsub2_rn(x, __hsub2_rn(sum, v)), __hsub2_rn(y, v));
+          b[u] = as_u32(r < 4 ? sum : rest);
+        }
+      }
+      mma(z, ph[0], pl[0], ph[1], pl[1], b[0], b[1]);
+    }
+    // ---- O += (p d) C: pairs of tokens (i, i + 4) and (i + 8, i + 12)
+    uint32_t vd[4][NG], vw[4][(NG + 1) / 2];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t vr = page + 10 * D + (4 * c + qi) * (D / 2);
+      lds_row<NG>(vh + (4 * c + qi) * (4 * NG), vd[c]);
+      if constexpr (NG == 4) {
+        lds(vr + (((2 * r) ^ (8 * (qi >> 1))) << 2), vw[c]);
+      } else {
+        if constexpr (NG >= 2) vw[c][0] = lds(vr + 4 * r);
+        if constexpr (NG & 1) vw[c][NG / 2] = lds_half(vr + ((NG - 1) * 8 + r) * 2);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const __half2 d = as_h2(prmt(vd[2 * u][g], vd[2 * u + 1][g], 0x5410u));
+        const __half2 p = as_h2(ph[u]), h = __hmul2(p, d);
+        hi[u] = as_u32(h);
+        lo[u] = EXACT ? as_u32(__hfma2(as_h2(pl[u]), d, __hfma2(p, d, __hneg2(h)))) : 0u;
+      }
+      const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+      const uint32_t b0 = prmt(vw[0][g / 2], vw[1][g / 2], sel), b1 = prmt(vw[2][g / 2], vw[3][g / 2], sel);
+      mma(o[g][0], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, false>(b0), codes<EXACT, 8, false>(b1));
+      mma(o[g][1], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, true>(b0), codes<EXACT, 8, true>(b1));
+      mma(o[g][2], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, false>(b0 >> 8), codes<EXACT, 8, false>(b1 >> 8));
+      mma(o[g][3], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, true>(b0 >> 8), codes<EXACT, 8, true>(b1 >> 8));
     }
   }
 
+  // A page with keys that some row does not see: such keys weigh nothing, whatever they hold,
+  // so V headers that are not finite are zeroed, since 0 * NaN would reach every row of the
+  // MMA; a row that does see such a header gets its group's NaN here.
+  __device__ void sanitise(uint32_t vh, int key, int limit, float (&o)[NG][4][4]) const {
+    uint64_t nan_at = 0;
+#pragma unroll
+    for (int i = 0; i < (16 * NG + 31) / 32; ++i) {
+      const int at = 32 * i + lane;
+      bool no = false;
+      if (at < 16 * NG) {
+        const uint32_t h = lds(vh + 4 * at);
+        no = (h & 0x7c00u) == 0x7c00u || (h & 0x7c000000u) == 0x7c000000u;
+        if (no) asm volatile("st.shared.u32 [%0], %1;" ::"r"(vh + 4 * at), "r"(0u) : "memory");
+      }
+      nan_at |= (uint64_t)__ballot_sync(0xffffffffu, no) << (32 * i);
+    }
+    if (nan_at) {
+      const int cnt = max(0, min(kTok, limit - key));
+      for (int t = 0; t < cnt; ++t)
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+          if ((nan_at >> (t * NG + g)) & 1)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) o[g][p][0] = o[g][p][1] = NAN;
+    }
+    // the next bulk copy into this page follows these stores
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+  }
+
+  // Moves the sums to this lane's places in the join buffer (held: earlier ones are there, in
+  // terms of held_m) and the header sums to zs.
+  __device__ void flush(bool& held, float& held_m, float M, float (&o)[NG][4][4], float (&z)[4], float (&zs)[4]) const {
+    float* at = join + warp * kState + (lane >> 2) * kPitch + 8 * (lane & 3);
+    const float f = held ? ex2(held_m - M) : 0.0f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float4 v[2] = {};
+      if (held) {
+        v[0] = *reinterpret_cast<const float4*>(at + 32 * g);
+        v[1] = *reinterpret_cast<const float4*>(at + 32 * g + 4);
+      }
+      float* e = reinterpret_cast<float*>(v);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        e[p] = fmaf(e[p], f, o[g][p][0] + o[g][p][2]);
+        e[4 + p] = fmaf(e[4 + p], f, o[g][p][1] + o[g][p][3]);
+        o[g][p][0] = o[g][p][1] = o[g][p][2] = o[g][p][3] = 0.0f;
+      }
+      *reinterpret_cast<float4*>(at + 32 * g) = v[0];
+      *reinterpret_cast<float4*>(at + 32 * g + 4) = v[1];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      zs[c] = fmaf(zs[c], f, z[c]);
+      z[c] = 0.0f;
+    }
+    held = true;
+    held_m = M;
+  }
+
   // This warp's pages of the stretch: per row the running maximum M and sum l, and in
-  // fragments the products o and the header sums z.
-  __device__ void pages(Seg& sg, float& M, float& l, float (&o)[NG][4][4], float (&z)[4]) {
+  // fragments the products o (behind those already flushed, where `held`) and the header
+  // sums z.
+  __device__ void pages(Seg& sg, float& M, float& l, float (&o)[NG][4][4], float (&z)[4], bool& held) {
     const int qs = sg.qs, kvh = sg.kvh, mine = sg.mine, first = sg.first;
     const int row0 = sg.tile * kRows, rows = sg.nq * G;
     const int least = seen(sg, row0), most = seen(sg, min(row0 + kRows, rows) - 1);
@@ -588,7 +790,7 @@ struct Attn {
     const int row = row0 + r;
     const bool live = row < rows;
     const int limit = live ? seen(sg, row) : most;
-    uint32_t qm[2];
+    uint32_t qm[3] = {};
     float rowmul;
     {
       float x[NG][8], qsum[NG];
@@ -655,7 +857,12 @@ struct Attn {
           else
             q0 = qsum[g] * up;
         }
+      // (three parts: they meet minima of several steps, and their error would not average out)
       split(q0, q1, qm[0], qm[1]);
+      if constexpr (EXACT) {
+        const float2 h = __half22float2(as_h2(qm[0])), m = __half22float2(as_h2(qm[1]));
+        qm[2] = as_u32(__floats2half2_rn((q0 - h.x) - m.x, (q1 - h.y) - m.y));
+      }
     }
 
     const int kt = ((r & 1) << 2) | (r >> 1);  // token of S column r: columns 2 i, 2 i + 1 are tokens i, i + 4
@@ -666,14 +873,17 @@ struct Attn {
       const float headroom = attempt ? 0.0f : 8.0f, growth = attempt ? 0.0f : 12.0f;
       M = -1e30f;
       l = 0.0f;
+      held = false;
+      float held_m = 0.0f, zs[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) z[c] = 0.0f;
+      for (int c = 0; c < 4; ++c) z[c] = zs[c] = 0.0f;
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int p = 0; p < 4; ++p)
 #pragma unroll
           for (int c = 0; c < 4; ++c) o[g][p][c] = 0.0f;
+      int fresh = 0;  // pages since the last flush
       for (int j = 0; j < mine; ++j) {
         mbar_wait_bounded(bars + get, phase, a.status);
         const uint32_t page = ring32 + get * PB;
@@ -682,84 +892,17 @@ struct Attn {
           phase ^= 1;
         }
         const int key = (first + j * kAttnWarps) * kTok;
-        const bool partial = key + kTok > least;
         // ---- scores
-        uint64_t x2[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t kw[NG], h0[NG], h1[NG], hm[2] = {0, 0};
-          const uint32_t ph = page + 8 * D + 8 * u * (4 * NG);
-          lds_row<NG>(page + (8 * u + kt) * (D / 2) + qi * (4 * NG), kw);
-          lds_row<NG>(ph + qi * (4 * NG), h0);
-          lds_row<NG>(ph + (4 + qi) * (4 * NG), h1);
-          if constexpr (NG == 4) {
-            lds(ph + kt * 16 + 8 * (qi & 1), hm);
-          } else {
-            if (2 * qi < NG) hm[0] = lds(ph + kt * (4 * NG) + 8 * qi);
-            if (2 * qi + 1 < NG) hm[1] = lds(ph + kt * (4 * NG) + 8 * qi + 4);
-          }
-          float acc[4];
-          uint32_t bm = prmt(hm[0], hm[1], 0x7632u);
-          if (qi >= 2) bm = 0;
-          mma0(acc, qm[0], EXACT ? qm[1] : 0u, 0u, 0u, bm, 0u);
-          x2[u] = EXACT ? add2(f2(acc[0], acc[1]), f2(acc[2], acc[3])) : f2(acc[0], acc[1]);
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const uint32_t hw = kw[g] >> 8;
-            float e[4];
-            uint32_t qa[4];
-            lds(qfrag + g * 1024, qa);
-            mma0(e, qa[0], EXACT ? qa[1] : 0u, qa[2], EXACT ? qa[3] : 0u, codes<EXACT, 0, false>(kw[g]), codes<EXACT, 0, true>(kw[g]));
-            lds(qfrag + g * 1024 + 512, qa);
-            mma(e, qa[0], EXACT ? qa[1] : 0u, qa[2], EXACT ? qa[3] : 0u, codes<EXACT, 0, false>(hw), codes<EXACT, 0, true>(hw));
-            float d0 = __low2float(as_h2(h0[g])), d1 = __low2float(as_h2(h1[g]));
-            uint64_t sum = f2(e[0], e[1]);
-            if constexpr (EXACT) {
-              sum = add2(sum, f2(e[2], e[3]));
-            } else {
-              d0 *= 16777216.0f;  // the codes' 2^-24
-              d1 *= 16777216.0f;
-            }
-            x2[u] = fma2(f2(d0, d1), sum, x2[u]);
-          }
-        }
         float x[2][2];
-        *reinterpret_cast<float2*>(x[0]) = unf2(x2[0]);
-        *reinterpret_cast<float2*>(x[1]) = unf2(x2[1]);
-        const uint32_t vh = page + 18 * D;
-        if (partial) {
-          // Keys that a row does not see weigh nothing, whatever they hold: scores -inf, and
-          // V headers that are not finite zeroed, since 0 * NaN would reach every row of the
-          // MMA; a row that does see such a header gets its group's NaN here.
+#pragma unroll
+        for (int u = 0; u < 2; ++u) *reinterpret_cast<float2*>(x[u]) = unf2(scores(page, u, kt, qi, qm));
+        if (key + kTok > least) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int c = 0; c < 2; ++c)
               if (key + 8 * u + 4 * c + qi >= limit) x[u][c] = -INFINITY;
-          uint64_t nan_at = 0;
-#pragma unroll
-          for (int i = 0; i < (16 * NG + 31) / 32; ++i) {
-            const int at = 32 * i + lane;
-            bool no = false;
-            if (at < 16 * NG) {
-              const uint32_t h = lds(vh + 4 * at);
-              no = (h & 0x7c00u) == 0x7c00u || (h & 0x7c000000u) == 0x7c000000u;
-              if (no) asm volatile("st.shared.u32 [%0], %1;" ::"r"(vh + 4 * at), "r"(0u) : "memory");
-            }
-            nan_at |= (uint64_t)__ballot_sync(0xffffffffu, no) << (32 * i);
-          }
-          if (nan_at) {
-            const int cnt = max(0, min(kTok, limit - key));
-            for (int t = 0; t < cnt; ++t)
-#pragma unroll
-              for (int g = 0; g < NG; ++g)
-                if ((nan_at >> (t * NG + g)) & 1)
-#pragma unroll
-                  for (int p = 0; p < 4; ++p) o[g][p][0] = o[g][p][1] = NAN;
-          }
-          // the next bulk copy into this page follows these stores
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
+          sanitise(page + 18 * D, key, limit, o);
         }
         // ---- running softmax
         float mx = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])) * rowmul;
@@ -787,55 +930,36 @@ struct Attn {
           l += p0 + p1;
           const __half2 h = __floats2half2_rn(p0, p1);
           ph[u] = as_u32(h);
+          pl[u] = 0;
           if constexpr (EXACT) {
             const float2 f = __half22float2(h);
             pl[u] = as_u32(__floats2half2_rn(p0 - f.x, p1 - f.y));
-          } else {
-            pl[u] = 0;
           }
         }
-        // ---- sums of p times the minima (columns 0..3) and the steps (columns 4..7)
-        {
-          const int g = min(r & 3, NG - 1);
-          const uint32_t sel = r < 4 ? 0x7632u : 0x5410u;
-          const uint32_t at = vh + 4 * (qi * NG + g);
-          const uint32_t b0 = prmt(lds(at), lds(at + 16 * NG), sel), b1 = prmt(lds(at + 32 * NG), lds(at + 48 * NG), sel);
-          mma(z, ph[0], pl[0], ph[1], pl[1], b0, b1);
-        }
-        // ---- O += (p d) C: pairs of tokens (i, i + 4) and (i + 8, i + 12)
-        uint32_t vd[4][NG], vw[4][(NG + 1) / 2];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t vr = page + 10 * D + (4 * c + qi) * (D / 2);
-          lds_row<NG>(vh + (4 * c + qi) * (4 * NG), vd[c]);
-          if constexpr (NG == 4) {
-            lds(vr + (((2 * r) ^ (8 * (qi >> 1))) << 2), vw[c]);
-          } else {
-            if constexpr (NG >= 2) vw[c][0] = lds(vr + 4 * r);
-            if constexpr (NG & 1) vw[c][NG / 2] = lds_half(vr + ((NG - 1) * 8 + r) * 2);
-          }
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          uint32_t hi[2], lo[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const __half2 d = as_h2(prmt(vd[2 * u][g], vd[2 * u + 1][g], 0x5410u));
-            const __half2 p = as_h2(ph[u]), h = __hmul2(p, d);
-            hi[u] = as_u32(h);
-            lo[u] = EXACT ? as_u32(__hfma2(as_h2(pl[u]), d, __hfma2(p, d, __hneg2(h)))) : 0u;
-          }
-          const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
-          const uint32_t b0 = prmt(vw[0][g / 2], vw[1][g / 2], sel), b1 = prmt(vw[2][g / 2], vw[3][g / 2], sel);
-          mma(o[g][0], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, false>(b0), codes<EXACT, 8, false>(b1));
-          mma(o[g][1], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, true>(b0), codes<EXACT, 8, true>(b1));
-          mma(o[g][2], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, false>(b0 >> 8), codes<EXACT, 8, false>(b1 >> 8));
-          mma(o[g][3], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, true>(b0 >> 8), codes<EXACT, 8, true>(b1 >> 8));
-        }
+        values(page, attempt, r, qi, ph, pl, o, z);
         __syncwarp();
-        issue(sg, j + kStages);
+        if (j & 1) issue(sg, j + kStages - 1);  // the two pages just used
+        if constexpr (EXACT) {
+          // The tensor cores truncate their sums, always towards zero: over 50 pages that took
+          // 3e-6 of the output.  So the sums move, rounded, to shared memory now and then.
+          if (++fresh == kFlush) {
+            flush(held, held_m, M, o, z, zs);
+            fresh = 0;
+          }
+        }
       }
-      if (attempt || mine == 0) break;
+      if (held) {
+        flush(held, held_m, M, o, z, zs);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) z[c] = zs[c];
+      }
+      if (attempt) {
+        if constexpr (EXACT)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) z[c] *= 8.0f;
+        break;
+      }
+      if (mine == 0) break;
       float probe = 0.0f;
 #pragma unroll
       for (int g = 0; g < NG; ++g)
@@ -843,37 +967,49 @@ struct Attn {
         for (int p = 0; p < 4; ++p)
 #pragma unroll
           for (int c = 0; c < 4; ++c) probe = fmaf(o[g][p][c], 0.0f, probe);
+      if (held) {
+        const float* at = join + warp * kState + r * kPitch + 8 * qi;
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) probe = fmaf(at[32 * g + e], 0.0f, probe);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) probe = fmaf(z[c], 0.0f, probe);
       if (!__any_sync(0xffffffffu, probe != 0.0f)) break;  // NaN where anything was not finite
-      for (int j = 0; j < kStages; ++j) issue(sg, j);
+      // from the start once more: the ring is empty, and an odd number of pages may have used it
+      sg.ids = load_ids(sg, 0);
+      for (int j = 0; j < kStages; j += 2) issue(sg, j);
     }
   }
 
-  // Joins the warps' states and, where the unit goes on in other CTAs, the CTAs'.
-  __device__ void finish(const Place& w, const Seg& sg, int64_t begin, bool bad, float M, float l, const float (&o)[NG][4][4],
-                         const float (&z)[4]) {
+  // Joins the warps' states into the output or, where the unit goes on in other CTAs, into a
+  // part of it.
+  __device__ void finish(const Place& w, const Seg& sg, int64_t begin, float M, float l, const float (&o)[NG][4][4],
+                         const float (&z)[4], bool held, Open* left) {
     const int r = lane >> 2, qi = lane & 3;
     const int qs = sg.qs, kvh = sg.kvh, row0 = sg.tile * kRows, rows = sg.nq * G;
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (__any_sync(0xffffffffu, bad)) {  // a block id outside the pool: no number stands for these rows
+    if (__any_sync(0xffffffffu, sg.bad)) {  // a block id outside the pool: no number stands for these rows
       if (lane == 0) raise_status(a.status, kDevCache);
       l = NAN;
     }
     {
       float* out = join + warp * kState + r * kPitch + 8 * qi;
-      const float z0 = z[0] + z[2], z1 = z[1] + z[3];  // quad lanes 0, 1: minima; 2, 3: steps
+      const float z0 = z[0] + z[2], z1 = z[1] + z[3];  // quad lanes 0, 1: middles or minima; 2, 3: their rests
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const int from = (lane & ~3) + g / 2;
         const float zm = __shfl_sync(0xffffffffu, (g & 1) ? z1 : z0, from);
         const float zd = __shfl_sync(0xffffffffu, (g & 1) ? z1 : z0, from + 2);
-        const float zz = EXACT ? fmaf(8.0f, zd, zm) : zm;
+        const float zz = EXACT ? zm + zd : zm;
         float v[8];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           const float f = (EXACT ? 1.0f : 16777216.0f) * ((p & 1) ? 0.0625f : 1.0f);  // the odd nibbles' 16
-          v[p] = fmaf(o[g][p][0] + o[g][p][2], f, zz);
-          v[4 + p] = fmaf(o[g][p][1] + o[g][p][3], f, zz);
+          v[p] = fmaf(held ? out[32 * g + p] : o[g][p][0] + o[g][p][2], f, zz);
+          v[4 + p] = fmaf(held ? out[32 * g + 4 + p] : o[g][p][1] + o[g][p][3], f, zz);
         }
         *reinterpret_cast<float4*>(out + 32 * g) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4*>(out + 32 * g + 4) = make_float4(v[4], v[5], v[6], v[7]);
@@ -887,23 +1023,8 @@ struct Attn {
     const int tid = threadIdx.x;
     const int cta = blockIdx.x;
     const int c0 = (int)(begin / w.share), c1 = (int)((begin + sg.cost - 1) / w.share);
-    // a part: [8][D] sums, [8] maxima, [8] denominators
-    auto part = [&](int c) { return a.part + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * kPart; };
-    auto put = [&](int rr, int d, float4 v, float ls) {
-      const int rw = row0 + rr;
-      if (rw >= rows) return;
-      const float f = ls == 0.0f ? 0.0f : 1.0f / ls;
-      if (ls == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const int64_t at = (int64_t)(qs + rw / G) * a.ldo + (int64_t)(kvh * G + rw % G) * D + d;
-      if (a.o_wide && a.o_dtype == 0) {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-      } else {
-        store_from_f32(a.o, a.o_dtype, at, v.x * f);
-        store_from_f32(a.o, a.o_dtype, at + 1, v.y * f);
-        store_from_f32(a.o, a.o_dtype, at + 2, v.z * f);
-        store_from_f32(a.o, a.o_dtype, at + 3, v.w * f);
-      }
-    };
+    const Open u{qs, rows, kvh, row0, c0, c1, 0};
+    if (c0 != c1 && tid == 0) left[c0 == cta ? 1 : 0] = u;
     for (int e = tid; e < kRows * D / 4; e += kAttnThreads) {
       const int rr = e / (D / 4), d = 4 * (e - rr * (D / 4));
       const float* ml = join + kRows * kPitch + rr;
@@ -920,9 +1041,9 @@ struct Attn {
         os = make_float4(fmaf(v.x, f, os.x), fmaf(v.y, f, os.y), fmaf(v.z, f, os.z), fmaf(v.w, f, os.w));
       }
       if (c0 == c1) {
-        put(rr, d, os, ls);
+        put(u, rr, d, os, ls);
       } else {
-        float* p = part(cta);
+        float* p = part(u, cta);
         *reinterpret_cast<float4*>(p + rr * D + d) = os;
         if (d == 0) {
           p[kRows * D + rr] = m;
@@ -930,57 +1051,85 @@ struct Attn {
         }
       }
     }
-    if (c0 != c1) {  // the last CTA of the unit joins its parts, in CTA order
-      float* red = join + kJoinFloats;  // [2][4 warps][8], and the flag
-      int* last = reinterpret_cast<int*>(red + 2 * kAttnWarps * kRows);
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        *last = atomicAdd(a.count + c0, 1u) == (unsigned)(c1 - c0);
-        if (*last) a.count[c0] = 0;
-      }
-      __syncthreads();
-      if (*last) {
+    __syncthreads();  // the join buffer is used again
+  }
+
+  // a part: [8][D] sums, [8] maxima, [8] denominators
+  __device__ float* part(const Open& u, int c) const { return a.part + ((int64_t)c * 2 + (c == u.c0 ? 1 : 0)) * kPart; }
+  __device__ void put(const Open& u, int rr, int d, float4 v, float ls) const {
+    const int rw = u.row0 + rr;
+    if (rw >= u.rows) return;
+    const float f = ls == 0.0f ? 0.0f : 1.0f / ls;
+    if (ls == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int64_t at = (int64_t)(u.qs + rw / G) * a.ldo + (int64_t)(u.kvh * G + rw % G) * D + d;
+    if (a.o_wide && a.o_dtype == 0) {
+      *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+    } else {
+      store_from_f32(a.o, a.o_dtype, at, v.x * f);
+      store_from_f32(a.o, a.o_dtype, at + 1, v.y * f);
+      store_from_f32(a.o, a.o_dtype, at + 2, v.z * f);
+      store_from_f32(a.o, a.o_dtype, at + 3, v.w * f);
+    }
+  }
+
+  // The units that this CTA shares (the one begun before it, the one it leaves open): the last
+  // CTA of a unit to come here joins its parts, in CTA order.  Once, at the end of the CTA's
+  // stretch: the fence and the atomics cost 5 us a time.
+  __device__ void join_parts(Open* left) {
+    const int tid = threadIdx.x;
+    if (tid < 2) {
+      Open& u = left[tid];
+      u.last = 0;
+      if (u.c0 >= 0) {
         __threadfence();
-        // the parts' weights 2^(m_c - m), [c][8] in the join buffer: a thread takes a row
-        // and every 16th part
-        const int rr = tid & 7;
-        float m = -1e30f, ls = 0.0f;
-        for (int c = c0 + (tid >> 3); c <= c1; c += kAttnThreads / 8) {
-          const float v = __ldcg(part(c) + kRows * D + rr);
-          join[(c - c0) * kRows + rr] = v;
-          m = fmaxf(m, v);
-        }
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        if (lane < kRows) red[warp * kRows + rr] = m;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kAttnWarps; ++k) m = fmaxf(m, red[k * kRows + rr]);
-        for (int c = c0 + (tid >> 3); c <= c1; c += kAttnThreads / 8) {
-          const float f = ex2(join[(c - c0) * kRows + rr] - m);
-          join[(c - c0) * kRows + rr] = f;
-          ls = fmaf(__ldcg(part(c) + kRows * D + kRows + rr), f, ls);
-        }
-        ls += __shfl_xor_sync(0xffffffffu, ls, 8);
-        ls += __shfl_xor_sync(0xffffffffu, ls, 16);
-        if (lane < kRows) red[(kAttnWarps + warp) * kRows + rr] = ls;
-        __syncthreads();
-        for (int e = tid; e < kRows * D / 4; e += kAttnThreads) {
-          const int er = e / (D / 4), d = 4 * (e - er * (D / 4));
-          float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-          for (int c = c0; c <= c1; ++c) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part(c) + er * D + d));
-            const float f = join[(c - c0) * kRows + er];
-            os = make_float4(fmaf(v.x, f, os.x), fmaf(v.y, f, os.y), fmaf(v.z, f, os.z), fmaf(v.w, f, os.w));
-          }
-          const float* lr = red + kAttnWarps * kRows + er;
-          put(er, d, os, (lr[0] + lr[kRows]) + (lr[2 * kRows] + lr[3 * kRows]));
-        }
+        u.last = atomicAdd(a.count + u.c0, 1u) == (unsigned)(u.c1 - u.c0);
+        if (u.last) a.count[u.c0] = 0;
+        __threadfence();
       }
     }
-    __syncthreads();  // the join buffer is used again
+    __syncthreads();
+    float* red = join + kJoinFloats;  // [2][4 warps][8]
+    for (int i = 0; i < 2; ++i) {
+      if (!left[i].last) continue;
+      const Open u = left[i];
+      // the parts' weights 2^(m_c - m), [c][8] in the join buffer: a thread takes a row and
+      // every 16th part
+      const int rr = tid & 7;
+      float m = -1e30f, ls = 0.0f;
+      for (int c = u.c0 + (tid >> 3); c <= u.c1; c += kAttnThreads / 8) {
+        const float v = __ldcg(part(u, c) + kRows * D + rr);
+        join[(c - u.c0) * kRows + rr] = v;
+        m = fmaxf(m, v);
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      if (lane < kRows) red[warp * kRows + rr] = m;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kAttnWarps; ++k) m = fmaxf(m, red[k * kRows + rr]);
+      for (int c = u.c0 + (tid >> 3); c <= u.c1; c += kAttnThreads / 8) {
+        const float f = ex2(join[(c - u.c0) * kRows + rr] - m);
+        join[(c - u.c0) * kRows + rr] = f;
+        ls = fmaf(__ldcg(part(u, c) + kRows * D + kRows + rr), f, ls);
+      }
+      ls += __shfl_xor_sync(0xffffffffu, ls, 8);
+      ls += __shfl_xor_sync(0xffffffffu, ls, 16);
+      if (lane < kRows) red[(kAttnWarps + warp) * kRows + rr] = ls;
+      __syncthreads();
+      for (int e = tid; e < kRows * D / 4; e += kAttnThreads) {
+        const int er = e / (D / 4), d = 4 * (e - er * (D / 4));
+        float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int c = u.c0; c <= u.c1; ++c) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(part(u, c) + er * D + d));
+          const float f = join[(c - u.c0) * kRows + er];
+          os = make_float4(fmaf(v.x, f, os.x), fmaf(v.y, f, os.y), fmaf(v.z, f, os.z), fmaf(v.w, f, os.w));
+        }
+        const float* lr = red + kAttnWarps * kRows + er;
+        put(u, er, d, os, (lr[0] + lr[kRows]) + (lr[2 * kRows] + lr[3 * kRows]));
+      }
+      __syncthreads();
+    }
   }
 };
 
@@ -991,6 +1140,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) kv4_attn_kernel(cons
   __shared__ __align__(8) uint64_t bars[kAttnWarps][kStages];
   __shared__ int64_t sums[kAttnWarps];
   __shared__ Place place;
+  __shared__ typename Attn<NG, EXACT>::Seg next[kAttnWarps];
+  __shared__ typename Attn<NG, EXACT>::Open left[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Attn<NG, EXACT> at{a, smem + warp * (kStages * PB), smem_u32(smem + warp * (kStages * PB)), bars[warp], reinterpret_cast<float*>(smem + kAttnWarps * kStages * PB),
                      smem_u32(smem + kAttnWarps * kStages * PB + Attn<NG, EXACT>::kJoinBytes) + 16 * lane,
@@ -1038,7 +1189,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) kv4_attn_kernel(cons
     }
   __syncthreads();
   Place w = place;
-  at.run(w);
+  at.run(w, next + warp, left);
 }
 
 template <int NG, bool EXACT>
