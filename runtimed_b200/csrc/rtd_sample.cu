@@ -43,6 +43,8 @@ constexpr int kLanes = 4;    // threads that share an entry's comparisons
 constexpr int kCand = 1024;  // candidates that one CTA ranks
 constexpr int kMaxRanks = 8;
 constexpr int kNT = 512;
+constexpr int kWarps = kNT / 32;
+constexpr int kFar = 4;  // a chunk: so many of a lane's 16-byte vectors
 constexpr int kResident = 296;  // CTAs: more rows than fill the SMs get fewer CTAs each
 constexpr double kUnit = 17592186044416.0;  // 2^44
 
@@ -79,10 +81,9 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 
 struct Shared {
   uint32_t cnt[2][kBins], lo[2][kBins], hi[2][kBins];
-  // candidates of the row (in rank 0), or a bin's entries
-  uint32_t keys[kCand], idx[kCand];
+  uint64_t cand[kCand];  // candidates of the row (in rank 0): key << 32 | ~index
+  uint32_t keys[kCand];  // a bin's entries
   uint64_t weights[kCand];
-  uint32_t place[kCand];
   uint32_t list[kList + 1];
   uint64_t red[32];
   uint64_t red2[32];
@@ -91,16 +92,16 @@ struct Shared {
   uint32_t found, found_cnt;
   uint64_t found_above, found_total;
   double pow2[64];            // 2^(44 - i / 64)
-  float queue[32][64];        // kept values waiting for a full warp of exponentials
+  float queue[kWarps][64];     // kept values waiting for a full warp of exponentials
+  uint16_t hits[kWarps][64];   // chunks waiting to be looked at
+  __nv_bfloat16 marks[];       // the chunks' maxima, rounded up
 };
 
-template <int DT, int NT>
+template <int DT>
 struct Row {
-  static constexpr int kWarps = NT / 32;
-  static constexpr int kPer = kBins / NT;       // bins, or candidates, of a thread
+  static constexpr int kPer = kBins / kNT;       // bins, or candidates, of a thread
   static constexpr int kVec = DT == 0 ? 4 : 8;  // entries of 16 bytes
-  static constexpr int kAhead = DT == 0 ? 4 : 2;  // loads in flight where every entry is looked at,
-  static constexpr int kFar = 4;                  // and where few are
+  static constexpr int kAhead = DT == 0 ? 4 : 2;  // loads in flight where every entry is looked at
   const SampleArgs& a;
   Shared& sm;
   cg::cluster_group cluster;
@@ -131,8 +132,9 @@ struct Row {
     const double w = fma(__hiloint2double(__double2hiint(f) - ((i >> 6) << 20), __double2loint(f)), e, 4503599627370496.0);
     return (uint64_t)__double_as_longlong(w) & 0xFFFFFFFFFFFFFull;  // rounded, in the mantissa under 2^52
   }
-  // miss(value) for every entry, then f(value, weight) for those above `low`: where that is
-  // not all, few lanes of a warp hold one, and they wait for a full warp of exponentials.
+  // miss(value) at least for the entries that are not below `low`, and f(value, weight) for those
+  // above it: where that is not all, few lanes of a warp hold one, and they wait for a full warp
+  // of exponentials.
   template <typename F, typename G>
   __device__ void weigh(float low, G miss, F f) {
     if (low == -INFINITY) {
@@ -141,7 +143,7 @@ struct Row {
     }
     float* q = sm.queue[warp];
     int waiting = 0;
-    each<1>([&](int, float v) {
+    each_from(low, [&](int, float v) {
       miss(v);
       const bool in = v > low;
       const uint32_t late = __ballot_sync(0xffffffffu, in);
@@ -240,43 +242,74 @@ struct Row {
     }
   }
 
-  // f(largest of a few entries), covering this warp's; NaN counts for nothing.
-  template <typename F>
-  __device__ void each_max(F f) const {
+  __device__ __nv_bfloat16* marks_of_warp() const { return sm.marks + warp * (chunk_steps(a.per_warp) * 32); }
+  // Steps of a chunk a lane over n entries.
+  __host__ __device__ static constexpr int chunk_steps(int n) { return (n + kFar * 32 * kVec - 1) / (kFar * 32 * kVec); }
+
+  // The largest of this lane's entries that is no NaN; leaves the chunks' maxima in marks.
+  __device__ float row_max() const {
+    float most = -INFINITY;
     if (a.wide) {
+      __nv_bfloat16* mark = marks_of_warp() + lane;
 #pragma unroll 1
-      for (int i = w0 + lane * kVec; i - lane * kVec < w1; i += kFar * 32 * kVec) {
+      for (int i = w0 + lane * kVec; i - lane * kVec < w1; i += kFar * 32 * kVec, mark += 32) {
         uint4 q[kFar];
 #pragma unroll
         for (int k = 0; k < kFar; ++k) q[k] = raw_at(i + k * 32 * kVec);
+        float m = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < kFar; ++k) f(largest(q[k]));
+        for (int k = 0; k < kFar; ++k) m = fmaxf(m, largest(q[k]));
+        *mark = __float2bfloat16_ru(m);
+        most = fmaxf(most, m);
       }
     } else {
-      for (int i = w0 + lane; i < w1; i += 32) f(load<DT>(x, i));
+      for (int i = w0 + lane; i < w1; i += 32) most = fmaxf(most, load<DT>(x, i));
     }
+    return most;
   }
-  // f(index, value) at least for the entries that are not below `low` (few of them).
+  // f(index, value) at least for the entries that are not below `low`, the whole warp in every
+  // call (lanes without an entry bring NaN).  The marks tell which chunks hold any; 32 of those
+  // at a time are shared out, a vector of eight of them a lane.
   template <typename F>
   __device__ void each_from(float low, F f) const {
-    if (a.wide) {
+    if (!a.wide) {
+      each<1>(f);
+      return;
+    }
+    const __nv_bfloat16* mark = marks_of_warp() + lane;
+    uint16_t* hits = sm.hits[warp];
+    const int steps = chunk_steps(w1 - w0);
+    int waiting = 0;
 #pragma unroll 1
-      for (int i = w0 + lane * kVec; i - lane * kVec < w1; i += kFar * 32 * kVec) {
+    for (int it = 0; it <= steps; ++it) {
+      const bool in = it < steps && __bfloat162float(mark[it < steps ? it * 32 : 0]) >= low;
+      const uint32_t late = __ballot_sync(0xffffffffu, in);
+      if (in) hits[waiting + __popc(late & ((1u << lane) - 1u))] = (uint16_t)(it * 32 + lane);
+      waiting += __popc(late);
+      __syncwarp();
+      if (waiting >= 32 || (it == steps && waiting > 0)) {
         uint4 q[kFar];
+        int at[kFar];
 #pragma unroll
-        for (int k = 0; k < kFar; ++k) q[k] = raw_at(i + k * 32 * kVec);
+        for (int k = 0; k < kFar; ++k) {
+          const int n = (lane >> 2) + 8 * k, chunk = hits[n];
+          at[k] = n < waiting ? w0 + ((chunk >> 5) * (kFar * 32) + (lane & 3) * 32 + (chunk & 31)) * kVec : w1;
+          q[k] = raw_at(at[k]);
+        }
 #pragma unroll
-        for (int k = 0; k < kFar; ++k)
-          if (largest(q[k]) >= low) {
-            float v[kVec];
-            unpack(q[k], v);
+        for (int k = 0; k < kFar; ++k) {
+          if (8 * k >= waiting || !__any_sync(0xffffffffu, largest(q[k]) >= low)) continue;
+          float v[kVec];
+          unpack(q[k], v);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e)
-              if (v[e] >= low) f(i + k * 32 * kVec + e, v[e]);
-          }
+          for (int e = 0; e < kVec; ++e) f(at[k] + e, v[e]);
+        }
+        waiting = max(0, waiting - 32);
+        const uint16_t next = hits[32 + lane];
+        __syncwarp();
+        hits[lane] = next;
+        __syncwarp();
       }
-    } else {
-      for (int i = w0 + lane; i < w1; i += 32) f(i, load<DT>(x, i));
     }
   }
 
@@ -354,7 +387,7 @@ struct Row {
   }
 
   __device__ void clear_hist(int b) {
-    for (int i = tid; i < kBins; i += NT) sm.cnt[b][i] = sm.lo[b][i] = sm.hi[b][i] = 0;
+    for (int i = tid; i < kBins; i += kNT) sm.cnt[b][i] = sm.lo[b][i] = sm.hi[b][i] = 0;
   }
 
   template <bool W>
@@ -444,19 +477,19 @@ struct Row {
     for (int r = 0; r < ranks; ++r) {
       const Shared* o = cluster.map_shared_rank(&sm, r);
       const uint32_t m = min(o->list_n, (uint32_t)kList);
-      for (uint32_t i = tid; i < m && total + i < (uint32_t)kCand; i += NT) sm.keys[total + i] = o->list[i];
+      for (uint32_t i = tid; i < m && total + i < (uint32_t)kCand; i += kNT) sm.keys[total + i] = o->list[i];
       total += m;
     }
     if (tie_in && tid == 0 && total < (uint32_t)kCand) sm.keys[total] = tie_key;
     if (tie_in) ++total;
     total = min(total, (uint32_t)kCand);
     __syncthreads();
-    for (uint32_t i = tid; i < total; i += NT) {
+    for (uint32_t i = tid; i < total; i += kNT) {
       const uint64_t w = W ? weight(value_of(sm.keys[i])) : 1;
       sm.weights[i] = (tie_in && i == total - 1) ? ties * w : w;
     }
     __syncthreads();
-    for (uint32_t i0 = 0; i0 < total; i0 += NT / kLanes) {
+    for (uint32_t i0 = 0; i0 < total; i0 += kNT / kLanes) {
       const uint32_t i = i0 + tid / kLanes;
       const uint32_t k = i < total ? sm.keys[i] : 0;
       uint64_t gt = 0, eq = 0;
@@ -629,47 +662,80 @@ struct Row {
     return e >= 1.0 ? min(total, (uint64_t)e) : 1;
   }
 
-  // The k largest are among n <= kCand candidates: rank 0 decides on them alone.
-  __device__ void among(int n, int k, float p, uint64_t least, float u, int row) {
-    const int most = min(n, k);
-    // ranks, and the weights in order of rank
-    for (int i0 = 0; i0 < n; i0 += NT / kLanes) {
-      const int i = i0 + tid / kLanes;
-      const uint32_t key = i < n ? sm.keys[i] : 0, id = i < n ? sm.idx[i] : 0;
-      uint32_t place = 0;
+  // Sorts n <= kCand different values above zero (in shared memory, complete), the largest first.
+  // Up to 128 by counting the larger ones, kLanes threads a value: 0.4 us there against 1.0;
+  // more by a bitonic network on the next power of two, whose steps of up to 32 places stay
+  // within a warp's 64 values: for 265, 1.5 us against 10.
+  template <typename U>
+  __device__ void sort(U* v, int n) const {
+    if (n <= kNT / kLanes) {
+      const int i = tid / kLanes;
+      const U x = i < n ? v[i] : 0;
+      int place = 0;
 #pragma unroll 4
-      for (int j = tid % kLanes; j < n; j += kLanes) {
-        const uint32_t kj = sm.keys[j];
-        place += kj > key || (kj == key && sm.idx[j] < id);
-      }
+      for (int j = tid % kLanes; j < n; j += kLanes) place += v[j] > x;
 #pragma unroll
       for (int o = 1; o < kLanes; o *= 2) place += __shfl_xor_sync(0xffffffffu, place, o);
-      if (i < n && tid % kLanes == 0) {
-        sm.place[i] = place;
-        sm.weights[place] = place < (uint32_t)most ? weight(value_of(key)) : 0;
+      __syncthreads();
+      if (i < n && tid % kLanes == 0) v[place] = x;
+      __syncthreads();
+      return;
+    }
+    const int all = 1 << (32 - __clz(n - 1));
+    for (int i = n + tid; i < all; i += kNT) v[i] = 0;
+    __syncthreads();
+    for (int size = 2; size <= all; size *= 2)
+      for (int j = size / 2; j > 0; j /= 2) {
+        if (tid < all / 2) {
+          const int i = 2 * tid - (tid & (j - 1));
+          const U x = v[i], y = v[i + j];
+          if ((x < y) == ((i & size) == 0)) {
+            v[i] = y;
+            v[i + j] = x;
+          }
+        }
+        if (j > 32 || (j == 1 && size > 32))
+          __syncthreads();
+        else
+          __syncwarp();
       }
+  }
+
+  // The sum of the threads' values before this one's, and of all.
+  __device__ uint64_t scan(uint64_t mine, uint64_t& total) const {
+    uint64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
     }
     __syncthreads();
-    uint64_t w[kPer], mine = 0;
+    if (lane == 31) sm.red[warp] = inc;
+    __syncthreads();
+    uint64_t before = lane < warp ? sm.red[lane] : 0;
+    total = lane < kWarps ? sm.red[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    return before + inc - mine;
+  }
+
+  // The k largest are among n <= kCand candidates: rank 0 decides on them alone.  Two sorts: by
+  // rank for the filters, which each keep the first so many, and those by index for the pick.
+  __device__ void among(int n, int k, float p, uint64_t least, float u, int row) {
+    const int most = min(n, k);
+    sort(sm.cand, n);
+    uint64_t w[kPer], mine = 0, total;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      w[e] = kPer * tid + e < most ? sm.weights[kPer * tid + e] : 0;
+      const int r = kPer * tid + e;
+      w[e] = r < most ? weight(value_of((uint32_t)(sm.cand[r] >> 32))) : 0;
       mine += w[e];
     }
-    if (p < 1.0f) {  // in order of rank, those before which `enough` is not reached yet
-      uint64_t inc = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-      }
-      if (lane == 31) sm.red[warp] = inc;
-      __syncthreads();
-      uint64_t before = inc - mine, total = 0;
-      for (int e = 0; e < kWarps; ++e) {
-        if (e < warp) before += sm.red[e];
-        total += sm.red[e];
-      }
+    if (p < 1.0f) {  // those before which `enough` is not reached yet
+      uint64_t before = scan(mine, total);
       const uint64_t enough = nucleus(p, total);
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
@@ -677,26 +743,31 @@ struct Row {
         if (before >= enough) w[e] = 0;
         before = next;
       }
-      __syncthreads();
     }
-    mine = 0;
+    int kept = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       if (w[e] < least) w[e] = 0;
-      mine += w[e];
-      if (kPer * tid + e < n) sm.weights[kPer * tid + e] = w[e];
+      sm.weights[kPer * tid + e] = w[e];
+      kept += __syncthreads_count(w[e] > 0);
     }
-    const uint64_t at = drawn(u, block_sum(mine, sm.red));
-    // the pick, in index order
-    for (int i0 = 0; i0 < n; i0 += NT / kLanes) {
-      const int i = i0 + tid / kLanes;
-      const uint32_t id = i < n ? sm.idx[i] : 0;
-      uint64_t before = 0;
-#pragma unroll 4
-      for (int j = tid % kLanes; j < n; j += kLanes) before += sm.idx[j] < id ? sm.weights[sm.place[j]] : 0;
+    // the largest complement of (index, rank) first: the lowest index
+    for (int r = tid; r < kept; r += kNT) sm.keys[r] = ~((~(uint32_t)sm.cand[r] << 10) | (uint32_t)r);
+    __syncthreads();
+    sort(sm.keys, kept);
+    mine = 0;
 #pragma unroll
-      for (int o = 1; o < kLanes; o *= 2) before += __shfl_xor_sync(0xffffffffu, before, o);
-      if (i < n && tid % kLanes == 0 && before <= at && at < before + sm.weights[sm.place[i]]) a.ids[row] = (int)id;
+    for (int e = 0; e < kPer; ++e) {
+      const int r = kPer * tid + e;
+      w[e] = r < kept ? sm.weights[~sm.keys[r] & 1023u] : 0;
+      mine += w[e];
+    }
+    uint64_t before = scan(mine, total);
+    const uint64_t at = drawn(u, total);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (before <= at && at < before + w[e]) a.ids[row] = (int)(~sm.keys[kPer * tid + e] >> 10);
+      before += w[e];
     }
   }
 
@@ -707,8 +778,7 @@ struct Row {
     const float p = a.top_p ? a.top_p[row] : 1.0f;
     const float mp = a.min_p ? a.min_p[row] : 0.0f;
     const float u = a.u[row];
-    float mine = -INFINITY;
-    each_max([&](float v) { mine = fmaxf(mine, v); });
+    const float mine = row_max();
     uint64_t best = key_of(mine);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -732,7 +802,7 @@ struct Row {
     if (!(fabsf(top) < INFINITY) || !(t > 0.0f) || k == 1) {  // the maximum's lowest index
       uint32_t first = 0x7fffffffu;
       each_from(top, [&](int i, float v) {
-        if (v == top) first = min(first, (uint32_t)i);
+        if (v == top) first = min(first, (uint32_t)i);  // NaN past the row's end
       });
       first = __reduce_min_sync(0xffffffffu, first);
       if (lane == 0) atomicMin(&cluster.map_shared_rank(&sm, 0)->first, first);
@@ -751,7 +821,7 @@ struct Row {
       // The lanes' maxima bound the k-th largest from below: at least k entries lie in the
       // bins up to the one where the maxima reach k, and with many more lanes than k few
       // others do.
-      bool few = 2 * k <= ranks * NT;
+      bool few = 2 * k <= ranks * kNT;
       if (few) {
         if (mine > -INFINITY) atomicAdd(&sm.cnt[0][bin(mine)], 1u);
         cluster.sync();
@@ -768,10 +838,7 @@ struct Row {
         each_from(from, [&](int i, float v) {
           if (!((top - v) * c < upto)) return;
           const uint32_t at = atomicAdd(&o->cand_n, 1u);
-          if (at < (uint32_t)kCand) {
-            o->keys[at] = key_of(v);
-            o->idx[at] = (uint32_t)i;
-          }
+          if (at < (uint32_t)kCand) o->cand[at] = (uint64_t)key_of(v) << 32 | (uint32_t)~i;
         });
         cluster.sync();
         const uint32_t n = o->cand_n;
@@ -891,39 +958,44 @@ struct Row {
   }
 };
 
-template <int DT, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs a) {
+template <int DT>
+__global__ void __launch_bounds__(kNT, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sm = *reinterpret_cast<Shared*>(smem);
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = (int)(blockIdx.x / ranks);
   const int tid = threadIdx.x, warp = tid >> 5;
-  const int64_t first = (int64_t)(rank * (NT / 32) + warp) * a.per_warp;
+  const int64_t first = (int64_t)(rank * (kNT / 32) + warp) * a.per_warp;
   constexpr int es = DT == 0 ? 4 : 2;
-  Row<DT, NT> r{a, sm, cluster, static_cast<const uint8_t*>(a.x) + (int64_t)row * a.ldx * es, rank, ranks, tid, tid & 31, warp,
+  Row<DT> r{a, sm, cluster, static_cast<const uint8_t*>(a.x) + (int64_t)row * a.ldx * es, rank, ranks, tid, tid & 31, warp,
                 (int)min(first, (int64_t)a.V), (int)min(first + a.per_warp, (int64_t)a.V)};
   r.run(row);
   cluster.sync();  // no CTA leaves while another may read its shared memory
 }
 
-template <int DT, int NT>
+template <int DT>
+constexpr int smem_bytes(int per_warp) {
+  return (int)(sizeof(Shared) + kWarps * Row<DT>::chunk_steps(per_warp) * 32 * sizeof(__nv_bfloat16));
+}
+
+template <int DT>
 cudaError_t sample_launch(SampleArgs a, int64_t T, int ranks, cudaStream_t st) {
   static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (!(configured.load(std::memory_order_relaxed) & bit)) {
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel<DT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<DT>((int)(kSampleMaxVocab / kWarps)));
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int64_t warps = (int64_t)ranks * (NT / 32);
+  const int64_t warps = (int64_t)ranks * (kNT / 32);
   a.per_warp = (int)((a.V + warps - 1) / warps + 255) / 256 * 256;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(T * ranks));
-  cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.blockDim = dim3(kNT);
+  cfg.dynamicSmemBytes = smem_bytes<DT>(a.per_warp);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -932,7 +1004,7 @@ cudaError_t sample_launch(SampleArgs a, int64_t T, int ranks, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, sample_kernel<DT, NT>, a);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<DT>, a);
 }
 
 }  // namespace
@@ -946,7 +1018,7 @@ cudaError_t launch_sample(const void* x, int dt, int64_t ldx, int64_t T, int64_t
   const SampleArgs a{x, ldx, (int)V, 0, wide, temperature, top_k, top_p, min_p, u, ids};
   int ranks = 1;
   while (ranks < kMaxRanks && V > (int64_t)ranks * 4096 && 2 * ranks * T <= kResident) ranks *= 2;
-  return dt == 0 ? sample_launch<0, kNT>(a, T, ranks, st) : dt == 1 ? sample_launch<1, kNT>(a, T, ranks, st) : sample_launch<2, kNT>(a, T, ranks, st);
+  return dt == 0 ? sample_launch<0>(a, T, ranks, st) : dt == 1 ? sample_launch<1>(a, T, ranks, st) : sample_launch<2>(a, T, ranks, st);
 }
 
 }  // namespace rtd
