@@ -200,10 +200,15 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
 // A CTA serves one token (and a share of its heads when tokens are few): the rotation
 // angles pos * inv_freq[i] are formed and reduced in 64 bits once per CTA -- at position
 // 100000 a 32-bit angle is wrong by 6e-3 -- and their cosines and sines, rounded to f32,
-// serve every head.  A warp takes a head at a time, lane = dim within the group: the
-// group's extremes come from two warp reductions over order-mapped integers, whose ends
-// also reveal infinities and NaN.  Bound: HBM (x in, q and the pages out).
+// serve every head.  Queries whose whole head turns go by quads of neighbouring dims of
+// either half, asked for before the angles are formed.  Of the other heads a warp takes one
+// at a time, lane = dim within the group: the group's extremes come from two warp reductions
+// over order-mapped integers, whose ends also reveal infinities and NaN.
+// Bound: HBM.  2000 tokens of 64/8 heads of 128 in f32 move 161 MB, 25 us at the copy rate;
+// 44 us here, 59 with a lane per dim for the queries too (4-byte accesses).  The angles'
+// 64-bit sines hold up a CTA for 2 us, with four or five CTAs on an SM.
 constexpr int kAppThreads = 256;
+constexpr int kAppQuads = 2;  // 44 us as above; 1: 47; 4: 51, since fewer CTAs fit
 
 struct AppendArgs {
   const void* q;
@@ -211,6 +216,7 @@ struct AppendArgs {
   const void* v;
   int64_t ldq, ldk, ldv;
   int x_dtype;
+  int q_wide;  // queries in whole quads of both halves
   int n_head, n_kv, rot_dim;
   const double* inv_freq;
   const int* tok_pos;
@@ -244,25 +250,84 @@ __device__ __forceinline__ uint32_t quantise(float x, uint32_t& header) {
   return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, __half2float(m)), df)), 0.0f), 15.0f);
 }
 
+// Four neighbouring values: 16 bytes of f32 or 8 of 16 bits.
+__device__ __forceinline__ uint4 load_quad(const void* p, int dt, int64_t i) {
+  if (dt == 0) return *reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i);
+  const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+  return make_uint4(v.x, v.y, 0u, 0u);
+}
+__device__ __forceinline__ float4 quad_as_f32(uint4 v, int dt) {
+  if (dt == 0) return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+  float2 lo, hi;
+  if (dt == 1) {
+    lo = __half22float2(as_h2(v.x));
+    hi = __half22float2(as_h2(v.y));
+  } else {
+    lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
+    hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
+  }
+  return make_float4(lo.x, lo.y, hi.x, hi.y);
+}
+// A pair of dims turned by an angle, products rounded first, as rtd_rope_kv_append does.
+__device__ __forceinline__ void turn(float x, float y, float2 r, float& a, float& b) {
+  a = __fsub_rn(__fmul_rn(x, r.x), __fmul_rn(y, r.y));
+  b = __fadd_rn(__fmul_rn(y, r.x), __fmul_rn(x, r.y));
+}
+
 template <int NG>
 __global__ void __launch_bounds__(kAppThreads) rope_kv4_kernel(const AppendArgs a) {
   constexpr int D = 32 * NG;
-  __shared__ float2 cs[D / 2];
+  __shared__ __align__(16) float2 cs[D / 2];
   const int64_t t = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31;
   const int slot = __ldg(a.tok_slot + t), pos = __ldg(a.tok_pos + t);
   const int half = a.rot_dim / 2;
   const bool there = slot >= 0 && slot < a.num_slots;
   if (slot >= a.num_slots && tid == 0 && blockIdx.y == 0) raise_status(a.status, kDevCache);
+  // queries by quads of each half, if whole heads turn: kAppQuads are on their way before the
+  // angles are formed
+  constexpr int QD = D / 8;  // quads of a head's first half
+  const int quads = a.q_wide ? a.n_head * QD : 0, step = gridDim.y * kAppThreads;
+  int e = blockIdx.y * kAppThreads + tid;
+  uint4 qa[kAppQuads], qb[kAppQuads];
+  auto ask = [&]() {
+#pragma unroll
+    for (int k = 0; k < kAppQuads; ++k) {
+      const int i = e + k * step;
+      if (i >= quads) continue;
+      const int64_t at = t * a.ldq + (i / QD) * D + 4 * (i % QD);
+      qa[k] = load_quad(a.q, a.x_dtype, at);
+      qb[k] = load_quad(a.q, a.x_dtype, at + D / 2);
+    }
+  };
+  ask();
   for (int i = tid; i < half; i += kAppThreads) {
     double s, c;
     sincos((double)pos * a.inv_freq[i], &s, &c);
     cs[i] = make_float2((float)c, (float)s);
   }
   __syncthreads();
-  const int heads = a.n_head + 2 * a.n_kv;
-  const int warps = gridDim.y * (kAppThreads / 32);
-  for (int j = blockIdx.y * (kAppThreads / 32) + (tid >> 5); j < heads; j += warps) {
+  for (; e < quads; e += kAppQuads * step, ask()) {
+#pragma unroll
+    for (int k = 0; k < kAppQuads; ++k) {
+      const int i = e + k * step;
+      if (i >= quads) continue;
+      const float4 x = quad_as_f32(qa[k], a.x_dtype), y = quad_as_f32(qb[k], a.x_dtype);
+      const float4* r = reinterpret_cast<const float4*>(cs + 4 * (i % QD));
+      const float4 r0 = r[0], r1 = r[1];
+      float4 u, v;
+      turn(x.x, y.x, make_float2(r0.x, r0.y), u.x, v.x);
+      turn(x.y, y.y, make_float2(r0.z, r0.w), u.y, v.y);
+      turn(x.z, y.z, make_float2(r1.x, r1.y), u.z, v.z);
+      turn(x.w, y.w, make_float2(r1.z, r1.w), u.w, v.w);
+      float* out = a.q_out + (t * a.n_head + i / QD) * (int64_t)D + 4 * (i % QD);
+      *reinterpret_cast<float4*>(out) = u;
+      *reinterpret_cast<float4*>(out + D / 2) = v;
+    }
+  }
+  // the other heads a warp each, a lane per dim of a group
+  const int heads = a.n_head + 2 * a.n_kv, warps = gridDim.y * (kAppThreads / 32);
+  for (int j = (a.q_wide ? a.n_head : 0) + blockIdx.y * (kAppThreads / 32) + (tid >> 5); j < heads; j += warps) {
     const bool is_q = j < a.n_head, is_v = j >= a.n_head + a.n_kv;
     const int h = is_q ? j : (is_v ? j - a.n_head - a.n_kv : j - a.n_head);
     if (!is_q && !there) continue;
@@ -270,17 +335,27 @@ __global__ void __launch_bounds__(kAppThreads) rope_kv4_kernel(const AppendArgs 
     const int64_t base = t * (is_q ? a.ldq : (is_v ? a.ldv : a.ldk)) + (int64_t)h * D;
     float x[NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int d = 32 * g + lane;
-      float v = load_as_f32(src, a.x_dtype, base + d);
-      if (!is_v && d < 2 * half) {
-        const bool first = d < half;
-        const float o = load_as_f32(src, a.x_dtype, base + (first ? d + half : d - half));
-        const float2 r = cs[first ? d : d - half];
-        // products rounded first, as rtd_rope_kv_append does
-        v = first ? __fsub_rn(__fmul_rn(v, r.x), __fmul_rn(o, r.y)) : __fadd_rn(__fmul_rn(v, r.x), __fmul_rn(o, r.y));
+    for (int g = 0; g < NG; ++g) x[g] = load_as_f32(src, a.x_dtype, base + 32 * g + lane);
+    if (!is_v && NG % 2 == 0 && half == D / 2) {
+#pragma unroll
+      for (int g = 0; g < NG / 2; ++g) {
+        float u, v;
+        turn(x[g], x[g + NG / 2], cs[32 * g + lane], u, v);
+        x[g] = u;
+        x[g + NG / 2] = v;
       }
-      x[g] = v;
+    } else if (!is_v) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int d = 32 * g + lane;
+        if (d >= 2 * half) continue;
+        const float o = load_as_f32(src, a.x_dtype, base + (d < half ? d + half : d - half));
+        float u;
+        if (d < half)
+          turn(x[g], o, cs[d], x[g], u);
+        else
+          turn(o, x[g], cs[d - half], u, x[g]);
+      }
     }
     if (is_q) {
       float* out = a.q_out + (t * a.n_head + h) * (int64_t)D;
@@ -1244,7 +1319,9 @@ cudaError_t launch_rope_kv4(const void* q, int64_t ldq, const void* k, int64_t l
                             int x_dtype, int64_t T, int n_head, int n_kv, int head_dim, int rot_dim,
                             const double* inv_freq, const int* tok_pos, const int* tok_slot, uint8_t* pages,
                             int num_blocks, float* q_out, int sm_count, int* status, cudaStream_t st) {
-  AppendArgs a{q, k, v, ldq, ldk, ldv, x_dtype, n_head, n_kv, rot_dim, inv_freq, tok_pos, tok_slot, pages,
+  const int q_wide = rot_dim == head_dim && ldq % 4 == 0 && reinterpret_cast<uintptr_t>(q) % (x_dtype == 0 ? 16 : 8) == 0 &&
+                     reinterpret_cast<uintptr_t>(q_out) % 16 == 0;
+  AppendArgs a{q, k, v, ldq, ldk, ldv, x_dtype, q_wide, n_head, n_kv, rot_dim, inv_freq, tok_pos, tok_slot, pages,
                (int64_t)num_blocks * kTok, q_out, status};
   const int heads = n_head + 2 * n_kv, warps = kAppThreads / 32;
   const dim3 grid((unsigned)T, T < 2 * sm_count ? (unsigned)((heads + warps - 1) / warps) : 1u);
