@@ -581,12 +581,12 @@ struct Attn {
     nq = __ldg(a.q_start + s + 1) - qs;
     ctx = __ldg(a.ctx_len + s);
     bool bad = qs < 0 || nq < 0 || (int64_t)qs + nq > a.T || nq > a.max_q;
-    if (bad || nq * G >= a.wide_rows) nq = 0;
-    if (ctx > a.max_ctx) {
+    if (bad) nq = 0;
+    if (ctx < 0 || ctx > a.max_ctx) {
       bad |= nq > 0;
       ctx = 0;
     }
-    ctx = max(ctx, 0);
+    if (nq * G >= a.wide_rows) nq = 0;  // the wide kernel's, which leaves the telling to this one
     if (bad && tell) raise_status(a.status, kDevCache);
     return kUnitCost + (ctx + kTok - 1) / kTok;
   }

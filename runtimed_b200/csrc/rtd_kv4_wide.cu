@@ -625,8 +625,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
 template <int NG>
 cudaError_t wide_launch(const Kv4AttnArgs& a, int64_t ctas, int tiles, cudaStream_t st) {
   static std::atomic<uint64_t> configured{0};
+  static std::atomic<bool> fits{false};
   cudaError_t e = configure_once(kv4_wide_kernel<NG>, WidePlan<NG>::kSmem, configured);
   if (e != cudaSuccess) return e;
+  if (!fits.load(std::memory_order_relaxed)) {  // a split beyond the launch's registers would never start
+    cudaFuncAttributes at;
+    if ((e = cudaFuncGetAttributes(&at, kv4_wide_kernel<NG>)) != cudaSuccess) return e;
+    if (at.numRegs * kWideThreads < 32 * (kSoftWarps * kSoftRegs + kDecodeWarps * kDecodeRegs) + 128 * kOtherRegs)
+      return cudaErrorInvalidKernelImage;
+    fits.store(true, std::memory_order_relaxed);
+  }
   count_launch();
   kv4_wide_kernel<NG><<<(unsigned)ctas, kWideThreads, WidePlan<NG>::kSmem, st>>>(a, tiles);
   return cudaGetLastError();
