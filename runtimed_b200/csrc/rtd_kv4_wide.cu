@@ -139,7 +139,7 @@ __device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
 }
 
 template <int NG>
-__global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4AttnArgs a, int tiles) {
+__global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4AttnArgs a) {
   using P = WidePlan<NG>;
   constexpr int D = P::D, PB = P::PB;
   extern __shared__ uint8_t smem_raw[];
@@ -156,17 +156,50 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
   uint32_t* misc = reinterpret_cast<uint32_t*>(drained + 1);  // tensor-memory base, flags
   volatile uint32_t* abort_flag = misc + 1;
 
-  // ---- the unit: later row tiles see more keys and come first
+  // ---- the unit: the row tiles of the chunks in one list (the grid's bound on it counts T, not
+  // max_q, since one long chunk among many short sequences is the usual batch); of a sequence's
+  // the later ones see more keys and come first
+  __shared__ int sums[kWideThreads / 32], unit[2];
   const int G = a.n_head / a.n_kv;
-  unsigned bid = blockIdx.x;
-  const int kvh = (int)(bid % a.n_kv);
-  bid /= a.n_kv;
-  const int s = (int)(bid % a.S), tile = tiles - 1 - (int)(bid / a.S);
+  const int kvh = (int)(blockIdx.x % a.n_kv), want = (int)(blockIdx.x / a.n_kv);
+  auto row_tiles = [&](int s) {
+    const int qs = __ldg(a.q_start + s), nq = __ldg(a.q_start + s + 1) - qs;
+    if (qs < 0 || nq < 0 || (int64_t)qs + nq > a.T || nq > a.max_q) return 0;  // the other kernel tells
+    return nq * G < a.wide_rows ? 0 : (nq * G + 255) / 256;
+  };
+  {
+    const int per = (a.S + kWideThreads - 1) / kWideThreads;
+    const int s0 = min(a.S, (int)threadIdx.x * per), s1 = min(a.S, s0 + per);
+    int mine = 0;
+    for (int s = s0; s < s1; ++s) mine += row_tiles(s);
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if ((int)(threadIdx.x & 31) >= o) inc += y;
+    }
+    if ((threadIdx.x & 31) == 31) sums[threadIdx.x >> 5] = inc;
+    if (threadIdx.x == 0) unit[0] = -1;
+    __syncthreads();
+    for (int k = 0; k < (int)(threadIdx.x >> 5); ++k) inc += sums[k];
+    int before = inc - mine;
+    if (want >= before && want < inc)
+      for (int s = s0; s < s1; ++s) {
+        const int n = row_tiles(s);
+        if (want < before + n) {
+          unit[0] = s;
+          unit[1] = n - 1 - (want - before);
+          break;
+        }
+        before += n;
+      }
+    __syncthreads();
+  }
+  const int s = unit[0], tile = unit[1];
+  if (s < 0) return;
   const int qs = __ldg(a.q_start + s), nq = __ldg(a.q_start + s + 1) - qs;
   int ctx = __ldg(a.ctx_len + s);
-  if (qs < 0 || nq < 0 || (int64_t)qs + nq > a.T || nq > a.max_q) return;  // the other kernel tells
   const int rows = nq * G, row0 = tile * 256;
-  if (rows < a.wide_rows || row0 >= rows) return;
   if (ctx > a.max_ctx || ctx < 0) ctx = 0;
   auto seen = [&](int row) { return max(0, ctx - nq + row / G + 1); };
   const int least = seen(row0), most = seen(min(row0 + 256, rows) - 1);
@@ -623,7 +656,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
 }
 
 template <int NG>
-cudaError_t wide_launch(const Kv4AttnArgs& a, int64_t ctas, int tiles, cudaStream_t st) {
+cudaError_t wide_launch(const Kv4AttnArgs& a, int64_t ctas, cudaStream_t st) {
   static std::atomic<uint64_t> configured{0};
   static std::atomic<bool> fits{false};
   cudaError_t e = configure_once(kv4_wide_kernel<NG>, WidePlan<NG>::kSmem, configured);
@@ -636,16 +669,19 @@ cudaError_t wide_launch(const Kv4AttnArgs& a, int64_t ctas, int tiles, cudaStrea
     fits.store(true, std::memory_order_relaxed);
   }
   count_launch();
-  kv4_wide_kernel<NG><<<(unsigned)ctas, kWideThreads, WidePlan<NG>::kSmem, st>>>(a, tiles);
+  kv4_wide_kernel<NG><<<(unsigned)ctas, kWideThreads, WidePlan<NG>::kSmem, st>>>(a);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_kv4_wide(const Kv4AttnArgs& a, int head_dim, cudaStream_t st) {
-  const int64_t tiles = ((int64_t)a.max_q * (a.n_head / a.n_kv) + 255) / 256, ctas = tiles * a.n_kv * a.S;
+  // n rows have n / 256 whole tiles and a ragged one a chunk, whose chunks have wide_rows at least
+  const int64_t rows = (int64_t)a.T * (a.n_head / a.n_kv);
+  const int64_t ctas = (rows / 256 + std::min<int64_t>(a.S, rows / a.wide_rows)) * a.n_kv;
+  if (ctas == 0) return cudaSuccess;
   if (ctas > INT32_MAX) return cudaErrorInvalidConfiguration;
-  return head_dim == 128 ? wide_launch<4>(a, ctas, (int)tiles, st) : wide_launch<2>(a, ctas, (int)tiles, st);
+  return head_dim == 128 ? wide_launch<4>(a, ctas, st) : wide_launch<2>(a, ctas, st);
 }
 
 }  // namespace rtd
