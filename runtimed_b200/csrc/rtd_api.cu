@@ -816,7 +816,7 @@ rtd_status rtd_attention_kv4(rtd_ctx* ctx, const void* q, uint32_t q_dtype, int6
   if (!ctx) return fail(nullptr, RTD_ERR_INVALID, "%s: ctx is NULL", who);
   rtd_status st = check_heads4(ctx, n_head, n_kv, head_dim, who);
   if (st != RTD_OK) return st;
-  if (T < 0 || T > INT32_MAX || S < 0) return fail(ctx, RTD_ERR_SHAPE, "%s: T=%lld S=%d", who, (long long)T, S);
+  if (T < 0 || T > INT32_MAX / n_head || S < 0) return fail(ctx, RTD_ERR_SHAPE, "%s: T=%lld S=%d", who, (long long)T, S);
   if (T == 0 || S == 0) return RTD_OK;
   if (!q || !q_start || !ctx_len || !block_table || !o || max_blocks <= 0)
     return fail(ctx, RTD_ERR_INVALID, "%s: NULL pointer or no block table", who);

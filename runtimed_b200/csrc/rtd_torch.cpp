@@ -95,6 +95,7 @@ Pool pool(const at::Tensor& t) {
   const int64_t bytes = t.size(2), d = bytes / 20;
   if (bytes % 640 || d < 32 || d > 128)
     config_error("pages: " + std::to_string(bytes) + " bytes a page (20 times a head_dim of 32, 64, 96 or 128)");
+  if (t.size(1) < 1 || t.size(1) > INT32_MAX) config_error("pages: " + std::to_string(t.size(1)) + " kv heads");
   if (t.size(0) > INT32_MAX / 16) config_error("pages: more than 2^27 - 1 blocks");
   return Pool{t.size(0), t.size(1), d, t.device(), t.data_ptr()};
 }

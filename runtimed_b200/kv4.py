@@ -4,7 +4,8 @@ attention over the pages and a reader.
 Torch-level entry points of ``rtd_kv_plan``, ``rtd_rope_kv4_append``, ``rtd_attention_kv4``
 and ``rtd_kv4_read`` (``include/rtd.h`` states the format and the rules).  Each runs on the
 current stream of its tensors' device, allocates nothing but the outputs it returns, and
-may be captured in a CUDA graph.  ``BlockTables`` keeps the state that ``plan`` works on.
+may be captured in a CUDA graph.  ``attention`` works in its device's context: calls on two
+streams of a device, replayed graphs among them, must not overlap.  ``BlockTables`` keeps the state that ``plan`` works on.
 
 What only the device can see (a block id outside the pool, a length beyond its bound, an
 exhausted pool) is reported by ``Context.check_device_status``.

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from runtimed_b200 import kv4
+from runtimed_b200.errors import ConfigError
 from test_gpu_kv4 import Case, clean_status, dev, i32, run_attention, status  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -211,3 +212,33 @@ def test_equal_calls_another_stream_and_graphs():
         out.zero_()
         graphs[i % 2].replay()
         assert torch.equal(out, want[i % 3])
+
+
+@pytest.mark.parametrize("S,at", [(700, 350), (2000, 1999), (33, 0)])
+def test_a_long_chunk_among_many_short_sequences(S, at):
+    rng = np.random.default_rng(S)
+    lens, new = rng.integers(1, 40, S).tolist(), [1] * S
+    lens[at], new[at] = 300, 70
+    if S > at + 2:
+        lens[at + 2], new[at + 2] = 64, 12  # 96 rows: the least that is a chunk
+    c = Case(lens, 1, 64, seed=S)
+    check(c, new, 8)
+
+
+def test_no_tokens_and_no_heads():
+    c = Case([20], 2, 64, seed=1)
+    n = i32([])
+    none = torch.empty((0, 8, 64), device="cuda")
+    f = kv4.rope_frequencies(64, 1e4)
+    assert kv4.append(none, none[:, :2], none[:, :2], f, n, n, c.pages).shape == (0, 8, 64)
+    assert kv4.read(c.pages, n)[0].shape == (0, 2, 64)
+    assert kv4.attention(none, c.pages, i32(c.table), i32([0, 0]), i32([20]), 1, 20, out_dtype=torch.float16).shape == (0, 8, 64)
+    q = torch.ones((3, 8, 64), device="cuda")
+    out = torch.full((3, 8, 64), 2.0, device="cuda")
+    kv4.attention(q, c.pages, i32(np.zeros((0, 2))), i32([0]), n, 1, 20, out=out)  # no sequences
+    assert (out == 2.0).all()
+    headless = torch.zeros((4, 0, 1280), dtype=torch.uint8, device="cuda")
+    for call in (lambda: kv4.read(headless, n), lambda: kv4.attention(q, headless, i32(c.table), i32([0, 3]), i32([20]), 3, 20),
+                 lambda: kv4.append(q, q[:, :0], q[:, :0], f, n, n, headless)):
+        with pytest.raises(ConfigError):
+            call()

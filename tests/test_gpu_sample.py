@@ -196,3 +196,30 @@ def test_refusals():
         bad[at] = value
         assert L.rtd_sample(*bad) == code
     assert sampling.sample(x[:0], u[:0]).numel() == 0
+
+
+@pytest.mark.parametrize("T,k", [(2, 100), (2, 128), (2, 129), (2, 257), (2, 513), (2, 1000), (150, 129), (150, 256)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_sizes_of_top_k(T, k, dt):
+    # candidates counted (up to 128) and sorted (up to 1024), one CTA a row and eight; in bf16
+    # many are equal at the k-th place
+    V = 30000
+    x = logits(T, V, k).to(dt)
+    rng = np.random.default_rng(k)
+    for p, m in [(None, None), (0.97, 0.001)]:
+        f = lambda v: None if v is None else np.full(T, v)  # noqa: E731
+        check(x, rng.random(T, dtype=np.float32), rng.uniform(1.0, 4.0, T), f(k), f(p), f(m))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_the_largest_rows_one_cta_each(dt):
+    T, V, some = 150, 1 << 19, [0, 74, 149]
+    x = logits(3, V, 5).to(dt)
+    wide = torch.zeros((T, V), dtype=dt, device="cuda")
+    wide[some] = x.cuda()
+    u = np.random.default_rng(1).random(T, dtype=np.float32)
+    for k, p, m in [(50, 0.9, 0.01), (0, 0.9, 0.0), (0, 1.0, 0.0), (1, 1.0, 0.0)]:
+        full = lambda v, t: torch.full((T,), v, dtype=t, device="cuda")  # noqa: E731
+        got = sampling.sample(wide, torch.from_numpy(u).cuda(), None, full(k, torch.int32), full(p, torch.float32), full(m, torch.float32))
+        want = [pick(x[i].float().numpy(), u[r], 1.0, k, np.float64(np.float32(p)), np.float32(m)) for i, r in enumerate(some)]
+        assert got.cpu()[some].tolist() == want
