@@ -824,8 +824,9 @@ rtd_status rtd_attention_kv4(rtd_ctx* ctx, const void* q, uint32_t q_dtype, int6
   if (!valid_dtype(q_dtype) || !valid_dtype(o_dtype)) return fail(ctx, RTD_ERR_INVALID, "%s: bad dtype", who);
   if (ldq < (int64_t)n_head * head_dim || ldo < (int64_t)n_head * head_dim)
     return fail(ctx, RTD_ERR_SHAPE, "%s: row strides below n_head * head_dim", who);
-  if (max_ctx <= 0 || (max_ctx + 15ll) / 16 > max_blocks)
-    return fail(ctx, RTD_ERR_SHAPE, "%s: max_ctx %d outside the block table (%d blocks)", who, max_ctx, max_blocks);
+  if (max_ctx <= 0 || (max_ctx + 15ll) / 16 > max_blocks || max_blocks > INT32_MAX / 32)
+    return fail(ctx, RTD_ERR_SHAPE, "%s: max_ctx %d outside the block table (%d blocks, at most %d)", who, max_ctx, max_blocks,
+                INT32_MAX / 32);
   if (max_q <= 0) return fail(ctx, RTD_ERR_SHAPE, "%s: max_q %d", who, max_q);
   rtd::Kv4Attention c{q, (int)q_dtype, ldq, T, n_head, n_kv, head_dim, scale, q_start, ctx_len, S, block_table,
                       max_blocks, max_q, max_ctx, static_cast<const uint8_t*>(pages), num_blocks, o, (int)o_dtype, ldo,

@@ -447,12 +447,12 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const int* slots, int64_t
 // product as if its leading zeros counted, which costs 2e-5 of the output.
 //
 // Bound: 64 sequences of up to 4096 tokens, 64 query heads on 8 (f32 outputs) read 240 MB,
-// 37 us at the copy rate; the kernel takes 106 us (2.3 TB/s), 3 sequences of up to 60000 in
-// bf16 (184 MB, 28 us) 74 us.  It is the instructions: a page costs a warp 480 with f32 outputs, and the
-// three warps of a scheduler issue in 60 % of the cycles.  With the scores left out the
-// kernel took 80 us, with the values 85, with both 65.  Two CTAs an SM with rings of eight
-// pages and four with rings of three were no faster, nor was a loop over page pairs; five
-// stages took 110 us with f32 outputs and 75 in bf16.
+// 37 us at the copy rate; the kernel takes 104 us (2.3 TB/s), 3 sequences of up to 60000 in
+// bf16 (184 MB, 28 us) 69 us.  It is the instructions: a page costs a warp 480 with f32
+// outputs, and a scheduler with its three warps issues in 53 % of the cycles.  With the scores
+// left out an earlier version of 111 us took 80, with the values 85, with both 65.  Two CTAs
+// an SM with rings of eight pages and four with rings of three were no faster, nor was a loop
+// over page pairs; five stages cost 4 us with f32 outputs.
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
 constexpr int kStages = 4;  // even: pages are asked for in pairs (six do not fit three CTAs)
@@ -462,7 +462,12 @@ constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 512;
 // Sequences with so many rows (queries x heads of the group) run in the wide kernel.
 constexpr int kWideRows = 96;
-constexpr int kUnitCost = 8;  // what a unit costs beside its pages (queries, joins), in pages
+// What a unit costs beside its pages (queries, joins), in pages: 8 took 106 us for the first
+// of the cases above and 74 for the second, 16 takes 104 and 72, 24 the same.
+constexpr int kUnitCost = 16;
+// Units of up to so many pages are not split: the join costs 6 us (one sequence of 160 tokens:
+// 7 us whole, 13 split); 32 pages took 33 us for 8 sequences of 2000 and 4 queries, 16 31.
+constexpr int kWholePages = 16;
 
 __device__ __forceinline__ uint64_t f2(float a, float b) {
   uint64_t r;
@@ -548,14 +553,13 @@ struct Attn {
   static constexpr int kPitch = D + 4;                          // a row of a warp's state in the join buffer
   static constexpr int kState = kRows * kPitch + 2 * kRows;     // the rows, their maxima and denominators
   static constexpr int kPart = kRows * (D + 2);
-  static constexpr int kJoinFloats = kAttnWarps * kState > kMaxCtas * kRows ? kAttnWarps * kState : kMaxCtas * kRows;
-  static constexpr int kJoinBytes = (kJoinFloats + 2 * kAttnWarps * kRows + 4) * 4;
+  static constexpr int kJoinBytes = kAttnWarps * kState * 4;
   static constexpr int kSmem = kAttnWarps * kStages * PB + kJoinBytes + NG * 1024;
   const Kv4AttnArgs& a;
   uint8_t* ring;      // this warp's pages
   uint32_t ring32;
   uint64_t* bars;     // and their barriers
-  float* join;        // the warps' states, then the parts' weights
+  float* join;        // the warps' states
   uint32_t qfrag;     // this lane's query fragments, [group][k step][lane][16 bytes]
   int G, lane, warp;
   unsigned get = 0, phase = 0;  // the ring's next page to use, and its parity
@@ -1149,7 +1153,7 @@ struct Attn {
 
   // The units that this CTA shares (the one begun before it, the one it leaves open): the last
   // CTA of a unit to come here joins its parts, in CTA order.  Once, at the end of the CTA's
-  // stretch: the fence and the atomics cost 5 us a time.
+  // stretch: the fence and the atomics cost 3 us a time.
   __device__ void join_parts(Open* left) {
     const int tid = threadIdx.x;
     if (tid < 2) {
@@ -1163,47 +1167,41 @@ struct Attn {
       }
     }
     __syncthreads();
-    float* red = join + kJoinFloats;  // [2][4 warps][8]
     for (int i = 0; i < 2; ++i) {
       if (!left[i].last) continue;
       const Open u = left[i];
-      // the parts' weights 2^(m_c - m), [c][8] in the join buffer: a thread takes a row and
-      // every 16th part
-      const int rr = tid & 7;
-      float m = -1e30f, ls = 0.0f;
-      for (int c = u.c0 + (tid >> 3); c <= u.c1; c += kAttnThreads / 8) {
-        const float v = __ldcg(part(u, c) + kRows * D + rr);
-        join[(c - u.c0) * kRows + rr] = v;
-        m = fmaxf(m, v);
-      }
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-      if (lane < kRows) red[warp * kRows + rr] = m;
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kAttnWarps; ++k) m = fmaxf(m, red[k * kRows + rr]);
-      for (int c = u.c0 + (tid >> 3); c <= u.c1; c += kAttnThreads / 8) {
-        const float f = ex2(join[(c - u.c0) * kRows + rr] - m);
-        join[(c - u.c0) * kRows + rr] = f;
-        ls = fmaf(__ldcg(part(u, c) + kRows * D + kRows + rr), f, ls);
-      }
-      ls += __shfl_xor_sync(0xffffffffu, ls, 8);
-      ls += __shfl_xor_sync(0xffffffffu, ls, 16);
-      if (lane < kRows) red[(kAttnWarps + warp) * kRows + rr] = ls;
-      __syncthreads();
+      // a thread takes four dims of a row; the loads of eight parts do not wait for one another
       for (int e = tid; e < kRows * D / 4; e += kAttnThreads) {
         const int er = e / (D / 4), d = 4 * (e - er * (D / 4));
+        float m = -1e30f, ls = 0.0f;
         float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int c = u.c0; c <= u.c1; ++c) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(part(u, c) + er * D + d));
-          const float f = join[(c - u.c0) * kRows + er];
-          os = make_float4(fmaf(v.x, f, os.x), fmaf(v.y, f, os.y), fmaf(v.z, f, os.z), fmaf(v.w, f, os.w));
+        for (int c = u.c0; c <= u.c1; c += 8) {
+          float mc[8], lc[8];
+          float4 v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const bool in = c + k <= u.c1;
+            const float* p = part(u, in ? c + k : c);
+            mc[k] = in ? __ldcg(p + kRows * D + er) : -1e30f;
+            lc[k] = in ? __ldcg(p + kRows * D + kRows + er) : 0.0f;
+            v[k] = in ? __ldcg(reinterpret_cast<const float4*>(p + er * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+          float top = m;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top = fmaxf(top, mc[k]);
+          const float f = ex2(m - top);
+          m = top;
+          ls *= f;
+          os = make_float4(os.x * f, os.y * f, os.z * f, os.w * f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float w = ex2(mc[k] - top);
+            ls = fmaf(lc[k], w, ls);
+            os = make_float4(fmaf(v[k].x, w, os.x), fmaf(v[k].y, w, os.y), fmaf(v[k].z, w, os.z), fmaf(v[k].w, w, os.w));
+          }
         }
-        const float* lr = red + kAttnWarps * kRows + er;
-        put(u, er, d, os, (lr[0] + lr[kRows]) + (lr[2 * kRows] + lr[3 * kRows]));
+        put(u, er, d, os, ls);
       }
-      __syncthreads();
     }
   }
 };
@@ -1354,7 +1352,7 @@ cudaError_t launch_kv4_attention(const Kv4Attention& c) {
   const int wide_o = c.ldo % (c.o_dtype == 0 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(c.o) % 16 == 0;
   Kv4AttnArgs a{c.q, c.q_dtype, wide, c.ldq, (int)c.T, c.n_head, c.n_kv, c.scale, c.q_start, c.ctx_len, c.S, c.block_table,
                 c.max_blocks, c.max_q, c.max_ctx, c.pages, c.num_blocks, c.o, c.o_dtype, wide_o,
-                c.ldo, INT32_MAX, kUnitCost + std::min(32, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
+                c.ldo, INT32_MAX, kUnitCost + std::min(kWholePages, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
   const bool exact = c.o_dtype == 0;
   const int64_t rows = (int64_t)c.max_q * (c.n_head / c.n_kv);
   if (!exact && (c.head_dim == 64 || c.head_dim == 128) && rows >= kWideRows) {

@@ -8,8 +8,9 @@ import numpy as np
 import pytest
 import torch
 
-from runtimed_b200 import kv4
+from runtimed_b200 import _lib, kv4
 from runtimed_b200.errors import ConfigError
+from runtimed_b200.weights import Context
 from test_gpu_kv4 import Case, clean_status, dev, i32, run_attention, status  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -242,3 +243,15 @@ def test_no_tokens_and_no_heads():
                  lambda: kv4.append(q, q[:, :0], q[:, :0], f, n, n, headless)):
         with pytest.raises(ConfigError):
             call()
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    c = Case([20], 2, 64, seed=1)
+    L, h = _lib.lib(), Context.for_device("cuda:0").handle
+    p, f = c.pages.data_ptr(), torch.zeros((1, 8, 64), device="cuda").data_ptr()
+    z = torch.zeros(64, dtype=torch.int32, device="cuda").data_ptr()
+    att = [h, f, 0, 512, 1, 8, 2, 64, 0.1, z, z, 1, z, 2, 1, 20, p, 4, f, 0, 512, None]
+    for at, value in [(4, 2 ** 31 // 8), (13, 2 ** 26), (15, 33)]:  # T * heads, blocks of the table, max_ctx
+        bad = list(att)
+        bad[at] = value
+        assert L.rtd_attention_kv4(*bad) == _lib.RTD_ERR_SHAPE, (at, value)
