@@ -275,8 +275,9 @@ rtd_status rtd_kv4_read(rtd_ctx* ctx, const int32_t* slots, int64_t n, int32_t n
 /* Causal GQA over 4-bit pages.  Accuracy: an f32 output is that of exact codes with queries
  * and weights in 22 bits or more and 32-bit sums, about 1e-6 of the values.  A 16-bit output
  * takes queries and weights in 11 bits; sequences with 96 or more rows (queries x heads of the
- * group) at head_dim 64 or 128 also take keys and values rounded to f16, where those beyond
- * 65504 become infinite, and in them a row that sees a group of NaN values of one of the call's
+ * group) at head_dim 64 or 128, where they have 6144 or 4096 rows of queries x n_head in all,
+ * also take keys and values rounded to f16, where those beyond 65504 become infinite, and in
+ * them a row that sees a group of NaN values of one of the call's
  * own tokens may be NaN in all dims of the head.  Sequence s has the queries q_start[s] .. q_start[s + 1] - 1
  * (rows of q, ldq apart) at its last positions: the i-th of n sees the keys
  * 0 .. ctx_len[s] - n + i; a row that sees none is written as zeros, a row of no sequence

@@ -460,8 +460,14 @@ constexpr int kRows = 8;
 constexpr int kFlush = 16;  // pages a warp sums up on the tensor cores alone
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 512;
-// Sequences with so many rows (queries x heads of the group) run in the wide kernel.
+// Sequences with so many rows (queries x heads of the group) are prompt chunks: with 96 rows
+// the chunk kernel's 256-row tile is as fast as 12 tiles of 8 here if other chunks fill the GPU
+// (16 sequences of 2000, 64/8 heads of 128: 64 rows 66 us there, 111 here; 32 rows 66 and 63).
 constexpr int kWideRows = 96;
+// A chunk tile takes its time however few there are, so all chunks together need so many rows
+// (queries x n_head).  One sequence of 4000, 64/8 heads: of 128, 2048 rows take 98 us there and
+// 58 here, 4096 98 and 103; of 64, 4096 take 85 and 66, 8192 85 and 121.
+constexpr int64_t kWideTotal128 = 4096, kWideTotal64 = 6144;
 // What a unit costs beside its pages (queries, joins), in pages: 8 took 106 us for the first
 // of the cases above and 74 for the second, 16 takes 104 and 72, 24 the same.
 constexpr int kUnitCost = 16;
@@ -562,6 +568,7 @@ struct Attn {
   float* join;        // the warps' states
   uint32_t qfrag;     // this lane's query fragments, [group][k step][lane][16 bytes]
   int G, lane, warp;
+  int wide_rows = INT32_MAX;    // a.wide_rows where the chunks are many enough
   unsigned get = 0, phase = 0;  // the ring's next page to use, and its parity
   unsigned put_at = 0;          // the ring's next page to ask for
 
@@ -590,7 +597,7 @@ struct Attn {
       bad |= nq > 0;
       ctx = 0;
     }
-    if (nq * G >= a.wide_rows) nq = 0;  // the wide kernel's, which leaves the telling to this one
+    if (nq * G >= wide_rows) nq = 0;  // the wide kernel's, which leaves the telling to this one
     if (bad && tell) raise_status(a.status, kDevCache);
     return kUnitCost + (ctx + kTok - 1) / kTok;
   }
@@ -1226,6 +1233,19 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) kv4_attn_kernel(cons
   // ---- the line of work and this CTA's place on it
   const int per = (a.S + kAttnThreads - 1) / kAttnThreads;
   const int s0 = min(a.S, tid * per), s1 = min(a.S, s0 + per);
+  if (a.wide_rows < INT32_MAX) {
+    int64_t all = 0;
+    for (int s = s0; s < s1; ++s) all += chunk_rows(a, s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) sums[warp] = all;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int k = 0; k < kAttnWarps; ++k) all += sums[k];
+    __syncthreads();
+    if (all * a.n_kv >= a.wide_total) at.wide_rows = a.wide_rows;
+  }
   auto cost = [&](int s) -> int64_t {
     int qs, nq, ctx;
     const int unit = at.seq_info(s, qs, nq, ctx, blockIdx.x == 0);
@@ -1352,10 +1372,10 @@ cudaError_t launch_kv4_attention(const Kv4Attention& c) {
   const int wide_o = c.ldo % (c.o_dtype == 0 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(c.o) % 16 == 0;
   Kv4AttnArgs a{c.q, c.q_dtype, wide, c.ldq, (int)c.T, c.n_head, c.n_kv, c.scale, c.q_start, c.ctx_len, c.S, c.block_table,
                 c.max_blocks, c.max_q, c.max_ctx, c.pages, c.num_blocks, c.o, c.o_dtype, wide_o,
-                c.ldo, INT32_MAX, kUnitCost + std::min(kWholePages, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
+                c.ldo, INT32_MAX, c.head_dim == 128 ? kWideTotal128 : kWideTotal64, kUnitCost + std::min(kWholePages, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
   const bool exact = c.o_dtype == 0;
   const int64_t rows = (int64_t)c.max_q * (c.n_head / c.n_kv);
-  if (!exact && (c.head_dim == 64 || c.head_dim == 128) && rows >= kWideRows) {
+  if (!exact && (c.head_dim == 64 || c.head_dim == 128) && rows >= kWideRows && c.T * c.n_head >= a.wide_total) {
     a.wide_rows = kWideRows;
     cudaError_t e = launch_kv4_wide(a, c.head_dim, c.stream);
     if (e != cudaSuccess) return e;  // what follows is for the others, if any

@@ -91,12 +91,21 @@ struct Kv4AttnArgs {
   int o_dtype;
   int o_wide;       // rows on 16-byte boundaries
   int64_t ldo;
-  int wide_rows;    // sequences with at least so many rows (queries x G) are the wide kernel's
+  int wide_rows;    // sequences with at least so many rows (queries x G) are the wide kernel's,
+  int64_t wide_total;  // if all of these have so many (queries x n_head) together
   int min_share;    // pages a CTA takes at least
   float* part;      // [CTA][2][8 (D + 2)]: the units begun before it, and left open by it
   unsigned* count;  // [CTA]: parts done of the unit it leaves open, zero between calls
   int* status;
 };
+
+// A sequence's rows if it is a prompt chunk, else 0; what is wrong with it counts for nothing.
+__device__ __forceinline__ int chunk_rows(const Kv4AttnArgs& a, int s) {
+  const int qs = __ldg(a.q_start + s), nq = __ldg(a.q_start + s + 1) - qs;
+  if (qs < 0 || nq < 0 || (int64_t)qs + nq > a.T || nq > a.max_q) return 0;
+  const int rows = nq * (a.n_head / a.n_kv);
+  return rows < a.wide_rows ? 0 : rows;
+}
 
 // Prompt chunks (rtd_kv4_wide.cu): the sequences of at least a.wide_rows rows, 16-bit outputs,
 // head_dim 64 or 128.

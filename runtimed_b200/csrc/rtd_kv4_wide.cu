@@ -160,32 +160,41 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
   // max_q, since one long chunk among many short sequences is the usual batch); of a sequence's
   // the later ones see more keys and come first
   __shared__ int sums[kWideThreads / 32], unit[2];
+  __shared__ int64_t row_sums[kWideThreads / 32];
   const int G = a.n_head / a.n_kv;
   const int kvh = (int)(blockIdx.x % a.n_kv), want = (int)(blockIdx.x / a.n_kv);
-  auto row_tiles = [&](int s) {
-    const int qs = __ldg(a.q_start + s), nq = __ldg(a.q_start + s + 1) - qs;
-    if (qs < 0 || nq < 0 || (int64_t)qs + nq > a.T || nq > a.max_q) return 0;  // the other kernel tells
-    return nq * G < a.wide_rows ? 0 : (nq * G + 255) / 256;
-  };
   {
     const int per = (a.S + kWideThreads - 1) / kWideThreads;
     const int s0 = min(a.S, (int)threadIdx.x * per), s1 = min(a.S, s0 + per);
     int mine = 0;
-    for (int s = s0; s < s1; ++s) mine += row_tiles(s);
+    int64_t all = 0;
+    for (int s = s0; s < s1; ++s) {
+      const int n = chunk_rows(a, s);
+      mine += (n + 255) / 256;
+      all += n;
+    }
     int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, inc, o);
       if ((int)(threadIdx.x & 31) >= o) inc += y;
+      all += __shfl_xor_sync(0xffffffffu, all, o);
     }
-    if ((threadIdx.x & 31) == 31) sums[threadIdx.x >> 5] = inc;
+    if ((threadIdx.x & 31) == 31) {
+      sums[threadIdx.x >> 5] = inc;
+      row_sums[threadIdx.x >> 5] = all;
+    }
     if (threadIdx.x == 0) unit[0] = -1;
     __syncthreads();
-    for (int k = 0; k < (int)(threadIdx.x >> 5); ++k) inc += sums[k];
+    all = 0;
+    for (int k = 0; k < kWideThreads / 32; ++k) {
+      if (k < (int)(threadIdx.x >> 5)) inc += sums[k];
+      all += row_sums[k];
+    }
     int before = inc - mine;
-    if (want >= before && want < inc)
+    if (want >= before && want < inc && all * a.n_kv >= a.wide_total)
       for (int s = s0; s < s1; ++s) {
-        const int n = row_tiles(s);
+        const int n = (chunk_rows(a, s) + 255) / 256;
         if (want < before + n) {
           unit[0] = s;
           unit[1] = n - 1 - (want - before);
