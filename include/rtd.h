@@ -272,16 +272,17 @@ rtd_status rtd_rope_kv4_append(rtd_ctx* ctx, const void* q, int64_t ldq, const v
 rtd_status rtd_kv4_read(rtd_ctx* ctx, const int32_t* slots, int64_t n, int32_t n_kv, int32_t head_dim,
                         const void* pages, int32_t num_blocks, void* k, void* v, uint32_t dtype, void* stream);
 
-/* Causal GQA over 4-bit pages.  Accuracy: an f32 output is that of exact codes with queries
- * and weights in 22 bits or more and 32-bit sums, about 1e-6 of the values.  A 16-bit output
- * takes queries and weights in 11 bits; sequences with 96 or more rows (queries x heads of the
- * group) at head_dim 64 or 128, where they have 6144 or 4096 rows of queries x n_head in all,
- * also take keys and values rounded to f16, where those beyond 65504 become infinite, and in
- * them a row that sees a group of NaN values of one of the call's
- * own tokens may be NaN in all dims of the head.  Sequence s has the queries q_start[s] .. q_start[s + 1] - 1
+/* Causal GQA over 4-bit pages.  Sequence s has the queries q_start[s] .. q_start[s + 1] - 1
  * (rows of q, ldq apart) at its last positions: the i-th of n sees the keys
  * 0 .. ctx_len[s] - n + i; a row that sees none is written as zeros, a row of no sequence
  * is left alone.  max_q and max_ctx bound the queries and the length of any sequence.
+ * Accuracy: an f32 or f16 output is that of exact codes with queries and weights in 22 bits
+ * or more and 32-bit sums, about 1e-6 of the values before its own rounding; a bf16 output
+ * takes queries and weights in 11 bits.  With 16-bit outputs prompt chunks (sequences with
+ * 96 or more rows of queries x heads of the group, at head_dim 64 or 128, if they come to
+ * 6144 or 4096 rows of queries x n_head in all) take queries, weights, keys and values
+ * rounded to f16, where those beyond 65504 become infinite; a chunk's row that sees a NaN
+ * group of V among the call's own tokens may be NaN in all dims of the head.
  * o rows are ldo apart.  Long contexts are split over CTAs and joined in order, so equal
  * calls give equal bits.  A ctx_len outside 0 .. max_ctx counts as 0; a sequence with offsets
  * outside the T rows or with more than max_q queries is left alone; rows that read a block

@@ -436,15 +436,16 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const int* slots, int64_t
 // the minima's part as one more MMA over the groups.  For V the weights p * d_g multiply
 // the codes, and one MMA of p with the headers gives the minima's part.
 //
-// EXACT (f32 outputs): rows 0..7 of the 16-row MMA hold the f16 heads of q and p d, rows
+// EXACT (f32 and f16 outputs): rows 0..7 of the 16-row MMA hold the f16 heads of q and p d, rows
 // 8..15 the remainders, so that both enter with 22 bits (p d is split by an exact fma).  A
 // nibble masked into an f16 pair under the exponent of 1024 is 1024 + c (or 1024 + 16 c)
 // and one packed addition makes it c (16 c, against a 16th of the query), exactly; V takes
 // c - 8, so that a long mean of values near zero is a sum of both signs and not a
 // difference of two large ones.
-// Otherwise (16-bit outputs): the rows enter rounded to 11 bits and the nibble stays the
+// Otherwise (bf16 outputs): the rows enter rounded to 11 bits and the nibble stays the
 // f16 subnormal c * 2^-24, which saves the addition; the tensor cores align a subnormal's
-// product as if its leading zeros counted, which costs 2e-5 of the output.
+// product as if its leading zeros counted, which costs 2e-5 of the output.  f16 outputs were
+// 5e-4 off in this form, where rounding them costs 2e-4.
 //
 // Bound: 64 sequences of up to 4096 tokens, 64 query heads on 8 (f32 outputs) read 240 MB,
 // 37 us at the copy rate; the kernel takes 104 us (2.3 TB/s), 3 sequences of up to 60000 in
@@ -1373,9 +1374,9 @@ cudaError_t launch_kv4_attention(const Kv4Attention& c) {
   Kv4AttnArgs a{c.q, c.q_dtype, wide, c.ldq, (int)c.T, c.n_head, c.n_kv, c.scale, c.q_start, c.ctx_len, c.S, c.block_table,
                 c.max_blocks, c.max_q, c.max_ctx, c.pages, c.num_blocks, c.o, c.o_dtype, wide_o,
                 c.ldo, INT32_MAX, c.head_dim == 128 ? kWideTotal128 : kWideTotal64, kUnitCost + std::min(kWholePages, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
-  const bool exact = c.o_dtype == 0;
+  const bool exact = c.o_dtype != 2;  // bf16 rounds by 2^-9 what the other form rounds by 2^-11
   const int64_t rows = (int64_t)c.max_q * (c.n_head / c.n_kv);
-  if (!exact && (c.head_dim == 64 || c.head_dim == 128) && rows >= kWideRows && c.T * c.n_head >= a.wide_total) {
+  if (c.o_dtype != 0 && (c.head_dim == 64 || c.head_dim == 128) && rows >= kWideRows && c.T * c.n_head >= a.wide_total) {
     a.wide_rows = kWideRows;
     cudaError_t e = launch_kv4_wide(a, c.head_dim, c.stream);
     if (e != cudaSuccess) return e;  // what follows is for the others, if any
