@@ -448,9 +448,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const int* slots, int64_t
 // 5e-4 off in this form, where rounding them costs 2e-4.
 //
 // Bound: 64 sequences of up to 4096 tokens, 64 query heads on 8 (f32 outputs) read 240 MB,
-// 37 us at the copy rate; the kernel takes 104 us (2.3 TB/s), 3 sequences of up to 60000 in
-// bf16 (184 MB, 28 us) 69 us.  It is the instructions: a page costs a warp 480 with f32
-// outputs, and a scheduler with its three warps issues in 53 % of the cycles.  With the scores
+// 37 us at the copy rate; the kernel takes 97 us (2.5 TB/s), 3 sequences of up to 60000 in
+// bf16 (184 MB, 28 us) 69 us.  It is the instructions: a page costs a warp 450 with f32
+// outputs, and a scheduler with its three warps issues in half the cycles.  With the scores
 // left out an earlier version of 111 us took 80, with the values 85, with both 65.  Two CTAs
 // an SM with rings of eight pages and four with rings of three were no faster, nor was a loop
 // over page pairs; five stages cost 4 us with f32 outputs.
@@ -458,7 +458,6 @@ constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
 constexpr int kStages = 4;  // even: pages are asked for in pairs (six do not fit three CTAs)
 constexpr int kRows = 8;
-constexpr int kFlush = 16;  // pages a warp sums up on the tensor cores alone
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 512;
 // Sequences with so many rows (queries x heads of the group) are prompt chunks: with 96 rows
@@ -561,6 +560,7 @@ struct Attn {
   static constexpr int kState = kRows * kPitch + 2 * kRows;     // the rows, their maxima and denominators
   static constexpr int kPart = kRows * (D + 2);
   static constexpr int kJoinBytes = kAttnWarps * kState * 4;
+  static constexpr int kCols = EXACT ? 2 : 4;  // sums of a fragment: of both row halves, or as the MMA has them
   static constexpr int kSmem = kAttnWarps * kStages * PB + kJoinBytes + NG * 1024;
   const Kv4AttnArgs& a;
   uint8_t* ring;      // this warp's pages
@@ -689,9 +689,8 @@ struct Attn {
         }
         if (lane == 0) *next = n;
       }
-      float M, l, o[NG][4][4], z[4];
-      bool held;
-      pages(g, M, l, o, z, held);
+      float M, l, o[NG][4][kCols], z[4];
+      pages(g, M, l, o, z);
       const Seg done = g;
       if (more) {
         __syncwarp();
@@ -699,7 +698,7 @@ struct Attn {
         g.ids = ids;
         begin(g);
       }
-      finish(w, done, at, M, l, o, z, held, left);
+      finish(w, done, at, M, l, o, z, left);
       if (!more) break;
     }
     join_parts(left);
@@ -745,10 +744,25 @@ struct Attn {
     return x2;
   }
 
+  // o += hi C and lo C.  The tensor cores truncate their sums always towards zero, and codes
+  // about 8 lean to one side: summed there, 16 pages at a time, 13000 keys came out 2e-6 off.
+  // Added here, rounded, a page at a time, 4e-7, as sums in 32 bits throughout.
+  __device__ static void add(float (&o)[kCols], const uint32_t (&hi)[2], const uint32_t (&lo)[2], uint32_t b0, uint32_t b1) {
+    if constexpr (EXACT) {
+      float t[4];
+      mma0(t, hi[0], lo[0], hi[1], lo[1], b0, b1);
+      const float2 sum = unf2(add2(f2(o[0], o[1]), add2(f2(t[0], t[1]), f2(t[2], t[3]))));
+      o[0] = sum.x;
+      o[1] = sum.y;
+    } else {
+      mma(o, hi[0], lo[0], hi[1], lo[1], b0, b1);
+    }
+  }
+
   // O += (p d) C and the header sums z of a page, p = ph + pl of pairs of tokens (i, i + 4) and
   // (i + 8, i + 12).
   __device__ void values(uint32_t page, int attempt, int r, int qi, const uint32_t (&ph)[2], const uint32_t (&pl)[2],
-                         float (&o)[NG][4][4], float (&z)[4]) const {
+                         float (&o)[NG][4][kCols], float (&z)[4]) const {
     // ---- sums of p times what a group's codes add to: its minimum, or, about code 8, the
     // middle m + 8 d.  The middles lie around zero, where the sums of the minima and of the
     // steps would each grow and then cancel; column g takes the middle as f16, column 4 + g
@@ -770,7 +784,14 @@ struct Attn {
           b[u] = as_u32(r < 4 ? sum : rest);
         }
       }
-      mma(z, ph[0], pl[0], ph[1], pl[1], b[0], b[1]);
+      if constexpr (EXACT) {
+        float t[4];
+        mma0(t, ph[0], pl[0], ph[1], pl[1], b[0], b[1]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) z[c] += t[c];
+      } else {
+        mma(z, ph[0], pl[0], ph[1], pl[1], b[0], b[1]);
+      }
     }
     // ---- O += (p d) C: pairs of tokens (i, i + 4) and (i + 8, i + 12)
     uint32_t vd[4][NG], vw[4][(NG + 1) / 2];
@@ -797,17 +818,17 @@ struct Attn {
       }
       const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
       const uint32_t b0 = prmt(vw[0][g / 2], vw[1][g / 2], sel), b1 = prmt(vw[2][g / 2], vw[3][g / 2], sel);
-      mma(o[g][0], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, false>(b0), codes<EXACT, 8, false>(b1));
-      mma(o[g][1], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, true>(b0), codes<EXACT, 8, true>(b1));
-      mma(o[g][2], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, false>(b0 >> 8), codes<EXACT, 8, false>(b1 >> 8));
-      mma(o[g][3], hi[0], lo[0], hi[1], lo[1], codes<EXACT, 8, true>(b0 >> 8), codes<EXACT, 8, true>(b1 >> 8));
+      add(o[g][0], hi, lo, codes<EXACT, 8, false>(b0), codes<EXACT, 8, false>(b1));
+      add(o[g][1], hi, lo, codes<EXACT, 8, true>(b0), codes<EXACT, 8, true>(b1));
+      add(o[g][2], hi, lo, codes<EXACT, 8, false>(b0 >> 8), codes<EXACT, 8, false>(b1 >> 8));
+      add(o[g][3], hi, lo, codes<EXACT, 8, true>(b0 >> 8), codes<EXACT, 8, true>(b1 >> 8));
     }
   }
 
   // A page with keys that some row does not see: such keys weigh nothing, whatever they hold,
   // so V headers that are not finite are zeroed, since 0 * NaN would reach every row of the
   // MMA; a row that does see such a header gets its group's NaN here.
-  __device__ void sanitise(uint32_t vh, int key, int limit, float (&o)[NG][4][4]) const {
+  __device__ void sanitise(uint32_t vh, int key, int limit, float (&o)[NG][4][kCols]) const {
     uint64_t nan_at = 0;
 #pragma unroll
     for (int i = 0; i < (16 * NG + 31) / 32; ++i) {
@@ -834,41 +855,9 @@ struct Attn {
     __syncwarp();
   }
 
-  // Moves the sums to this lane's places in the join buffer (held: earlier ones are there, in
-  // terms of held_m) and the header sums to zs.
-  __device__ void flush(bool& held, float& held_m, float M, float (&o)[NG][4][4], float (&z)[4], float (&zs)[4]) const {
-    float* at = join + warp * kState + (lane >> 2) * kPitch + 8 * (lane & 3);
-    const float f = held ? ex2(held_m - M) : 0.0f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float4 v[2] = {};
-      if (held) {
-        v[0] = *reinterpret_cast<const float4*>(at + 32 * g);
-        v[1] = *reinterpret_cast<const float4*>(at + 32 * g + 4);
-      }
-      float* e = reinterpret_cast<float*>(v);
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        e[p] = fmaf(e[p], f, o[g][p][0] + o[g][p][2]);
-        e[4 + p] = fmaf(e[4 + p], f, o[g][p][1] + o[g][p][3]);
-        o[g][p][0] = o[g][p][1] = o[g][p][2] = o[g][p][3] = 0.0f;
-      }
-      *reinterpret_cast<float4*>(at + 32 * g) = v[0];
-      *reinterpret_cast<float4*>(at + 32 * g + 4) = v[1];
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      zs[c] = fmaf(zs[c], f, z[c]);
-      z[c] = 0.0f;
-    }
-    held = true;
-    held_m = M;
-  }
-
   // This warp's pages of the stretch: per row the running maximum M and sum l, and in
-  // fragments the products o (behind those already flushed, where `held`) and the header
-  // sums z.
-  __device__ void pages(Seg& sg, float& M, float& l, float (&o)[NG][4][4], float (&z)[4], bool& held) {
+  // fragments the products o and the header sums z.
+  __device__ void pages(Seg& sg, float& M, float& l, float (&o)[NG][4][kCols], float (&z)[4]) {
     const int qs = sg.qs, kvh = sg.kvh, mine = sg.mine, first = sg.first;
     const int row0 = sg.tile * kRows, rows = sg.nq * G;
     const int least = seen(sg, row0), most = seen(sg, min(row0 + kRows, rows) - 1);
@@ -960,17 +949,14 @@ struct Attn {
       const float headroom = attempt ? 0.0f : 8.0f, growth = attempt ? 0.0f : 12.0f;
       M = -1e30f;
       l = 0.0f;
-      held = false;
-      float held_m = 0.0f, zs[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) z[c] = zs[c] = 0.0f;
+      for (int c = 0; c < 4; ++c) z[c] = 0.0f;
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int p = 0; p < 4; ++p)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) o[g][p][c] = 0.0f;
-      int fresh = 0;  // pages since the last flush
+          for (int c = 0; c < kCols; ++c) o[g][p][c] = 0.0f;
       for (int j = 0; j < mine; ++j) {
         mbar_wait_bounded(bars + get, phase, a.status);
         const uint32_t page = ring32 + get * PB;
@@ -1007,7 +993,7 @@ struct Attn {
 #pragma unroll
               for (int p = 0; p < 4; ++p)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) o[g][p][c] *= f;
+                for (int c = 0; c < kCols; ++c) o[g][p][c] *= f;
           }
         }
         uint32_t ph[2], pl[2];
@@ -1026,19 +1012,6 @@ struct Attn {
         values(page, attempt, r, qi, ph, pl, o, z);
         __syncwarp();
         if (j & 1) issue(sg, j + kStages - 1);  // the two pages just used
-        if constexpr (EXACT) {
-          // The tensor cores truncate their sums, always towards zero: over 50 pages that took
-          // 3e-6 of the output.  So the sums move, rounded, to shared memory now and then.
-          if (++fresh == kFlush) {
-            flush(held, held_m, M, o, z, zs);
-            fresh = 0;
-          }
-        }
-      }
-      if (held) {
-        flush(held, held_m, M, o, z, zs);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) z[c] = zs[c];
       }
       if (attempt) {
         if constexpr (EXACT)
@@ -1053,14 +1026,7 @@ struct Attn {
 #pragma unroll
         for (int p = 0; p < 4; ++p)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) probe = fmaf(o[g][p][c], 0.0f, probe);
-      if (held) {
-        const float* at = join + warp * kState + r * kPitch + 8 * qi;
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) probe = fmaf(at[32 * g + e], 0.0f, probe);
-      }
+          for (int c = 0; c < kCols; ++c) probe = fmaf(o[g][p][c], 0.0f, probe);
 #pragma unroll
       for (int c = 0; c < 4; ++c) probe = fmaf(z[c], 0.0f, probe);
       if (!__any_sync(0xffffffffu, probe != 0.0f)) break;  // NaN where anything was not finite
@@ -1072,8 +1038,8 @@ struct Attn {
 
   // Joins the warps' states into the output or, where the unit goes on in other CTAs, into a
   // part of it.
-  __device__ void finish(const Place& w, const Seg& sg, int64_t begin, float M, float l, const float (&o)[NG][4][4],
-                         const float (&z)[4], bool held, Open* left) {
+  __device__ void finish(const Place& w, const Seg& sg, int64_t begin, float M, float l, const float (&o)[NG][4][kCols],
+                         const float (&z)[4], Open* left) {
     const int r = lane >> 2, qi = lane & 3;
     const int qs = sg.qs, kvh = sg.kvh, row0 = sg.tile * kRows, rows = sg.nq * G;
     l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -1095,8 +1061,8 @@ struct Attn {
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           const float f = (EXACT ? 1.0f : 16777216.0f) * ((p & 1) ? 0.0625f : 1.0f);  // the odd nibbles' 16
-          v[p] = fmaf(held ? out[32 * g + p] : o[g][p][0] + o[g][p][2], f, zz);
-          v[4 + p] = fmaf(held ? out[32 * g + 4 + p] : o[g][p][1] + o[g][p][3], f, zz);
+          v[p] = fmaf(o[g][p][0] + (EXACT ? 0.0f : o[g][p][kCols - 2]), f, zz);
+          v[4 + p] = fmaf(o[g][p][1] + (EXACT ? 0.0f : o[g][p][kCols - 1]), f, zz);
         }
         *reinterpret_cast<float4*>(out + 32 * g) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4*>(out + 32 * g + 4) = make_float4(v[4], v[5], v[6], v[7]);
