@@ -12,14 +12,17 @@
 //
 // A histogram over 1024 equal steps of (max - x) / t spreads any row's upper end over many
 // bins.  With top-k, the bins that hold the k largest usually hold few more: they are
-// gathered into one CTA, which ranks them against one another and decides alone.  Where
-// they are too many, and for a nucleus over the whole row, a select finds the exact
-// threshold: the bin where the count or weight is reached, then, if at most 512 entries
-// share it, their ranks, else splits of it by the bits of the value's order map.
+// gathered into one CTA, which sorts them and decides alone.  Where they are too many, and
+// for a nucleus over the whole row, a select finds the exact threshold: the bin where the
+// count or weight is reached, then, if at most 255 entries share it, their ranks, else splits
+// of it by the bits of the value's order map.
 //
 // Bound: for few rows the latency of the passes (three to five, the first from memory, the
-// others from L1) and of a cluster barrier after each; for many rows the 64-bit
-// exponentials of a nucleus over the whole row, else the passes' instructions.
+// others from L1) and of a cluster barrier after each: 1 row of 151936 with top-k 50 and top-p
+// 11 us.  64 rows of 152064 f32 with top-p alone take 74 us, of which in one row 4 the
+// maximum (at the memory's rate), 11 the histogram's shared-memory atomics, 18 the 64-bit
+// exponentials, and the steps between the passes 2 to 4 each.  200 rows in bf16 with every
+// filter take 27 us, 8 of them the maximum.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
