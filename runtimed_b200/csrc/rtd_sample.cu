@@ -830,8 +830,7 @@ struct Row {
         cluster.sync();
         find<false>([&](uint64_t total) { return total >= (uint64_t)k ? (uint64_t)k : 0; }, -1, 0, 0);
         few = sm.found_total >= (uint64_t)k && sm.found < (uint32_t)kBins - 1;
-        clear_hist(1);
-        buf = 1;
+        buf = 1;  // zero since the start: clearing it here would race with the select's counting, which may follow at once
       }
       if (few) {
         const float upto = (float)(sm.found + 1);

@@ -223,3 +223,25 @@ def test_the_largest_rows_one_cta_each(dt):
         got = sampling.sample(wide, torch.from_numpy(u).cuda(), None, full(k, torch.int32), full(p, torch.float32), full(m, torch.float32))
         want = [pick(x[i].float().numpy(), u[r], 1.0, k, np.float64(np.float32(p)), np.float32(m)) for i, r in enumerate(some)]
         assert got.cpu()[some].tolist() == want
+
+
+@pytest.mark.parametrize("T,k", [(2, 20), (2, 100), (2, 256), (150, 20), (150, 100), (150, 256)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_top_k_of_logits_that_few_threads_hold(T, k, dt):
+    # The largest lie side by side (a masked vocabulary) or far above the rest (a low temperature):
+    # the threads' maxima do not bound the k-th largest, and the histogram of the whole row follows
+    # at once.  Equal calls give equal ids, those of the rule.
+    V = 30000
+    rng = np.random.default_rng(k)
+    x = torch.full((T, V), -float("inf"))
+    x[:, 5000:5000 + 2 * k] = torch.from_numpy(rng.normal(0, 1, (T, 2 * k)).astype(np.float32))
+    low = logits(T, V, k)
+    for rows, t in [(x, None), (low, np.full(T, 0.02, np.float32))]:
+        rows = rows.to(dt)
+        for _ in range(3 if T < 10 else 1):
+            check(rows, rng.random(T, dtype=np.float32), t, np.full(T, k), np.full(T, 0.99), None)
+        d, u, kk = rows.cuda(), torch.from_numpy(rng.random(T, dtype=np.float32)).cuda(), torch.full((T,), k, dtype=torch.int32, device="cuda")
+        tt = None if t is None else torch.from_numpy(t).cuda()
+        first = sampling.sample(d, u, tt, kk)
+        for _ in range(50):
+            assert torch.equal(sampling.sample(d, u, tt, kk), first)
