@@ -176,7 +176,9 @@ rtd_status rtd_rmsnorm(rtd_ctx* ctx, float* h, int64_t ldh, const void* delta, u
 /* NeoX rope (crates/runtimed-model/src/ops/rope.rs:24-60) on the query and key heads of
  * the q / k / v linear outputs (f32), queries into q_out [T][n_head][head_dim] (f32), keys
  * and values appended to the paged cache at each token's (sequence, position):
- * SubstratePort::rope + Cache::append (crates/runtimed-model/src/arch/qwen2.rs:100-103). */
+ * SubstratePort::rope + Cache::append (crates/runtimed-model/src/arch/qwen2.rs:100-103).
+ * A row with a negative sequence or position (the padding of rtd_kv_plan's lists) writes no
+ * key or value; rtd_attention_paged writes zeros for a row with a negative position. */
 rtd_status rtd_rope_kv_append(rtd_ctx* ctx, const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v,
                               int64_t ldv, int64_t T, int32_t n_head, int32_t n_kv, int32_t head_dim, int32_t rot_dim,
                               float theta, const int32_t* tok_seq, const int32_t* tok_pos, const int32_t* block_table,

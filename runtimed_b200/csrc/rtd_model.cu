@@ -129,6 +129,7 @@ __global__ void rope_kv_kernel(const RopeArgs a) {
   const int half = a.rot_dim / 2;
   KV* kc = static_cast<KV*>(a.k_cache);
   KV* vc = static_cast<KV*>(a.v_cache);
+  if (j >= a.n_head && (seq < 0 || pos < 0)) return;  // a padded row has no place in the cache
   if (j >= a.n_head + a.n_kv) {  // value head: plain copy to the cache
     const int kvh = j - a.n_head - a.n_kv;
     const float* src = a.v + (int64_t)t * a.ldv + (int64_t)kvh * a.head_dim;

@@ -170,3 +170,48 @@ def test_a_step_without_free_blocks_is_reported(gguf):
     t.into(m.cache)
     assert m.cache.lengths == {0: 33, 3: 1} and len(m.cache._free) == 0
     Context.for_device("cuda:0").check_device_status()
+
+
+@pytest.mark.parametrize("kv", [torch.float16, torch.float32])
+def test_padded_rows_of_a_plan_leave_the_16_and_32_bit_caches_alone(kv):
+    # rtd_kv_plan pads its lists with -1 (all of them when it refuses): such a row appends nothing
+    # and its attention is zero, whichever cache the step runs on
+    from runtimed_b200 import _lib, kv4
+    from runtimed_b200.errors import ConfigError
+    from runtimed_b200.weights import Context
+
+    L, h, abi = _lib.lib(), Context.for_device("cuda:0"), _lib.DT_F16 if kv == torch.float16 else _lib.DT_F32
+    st = torch.cuda.current_stream().cuda_stream
+    rng = np.random.default_rng(0)
+    T, H, G, D = 6, 4, 2, 64
+    x = [torch.from_numpy(rng.normal(0, 1, (T, n * D)).astype(np.float32)).cuda() for n in (H, G, G)]
+
+    def run(t, T, max_ctx=32):
+        cache = [torch.full((5, G, 16, D), 3.0, dtype=kv, device="cuda") for _ in range(2)]
+        q, o = (torch.full((T, H * D), 9.0, device="cuda") for _ in range(2))
+        assert L.rtd_rope_kv_append(h.handle, x[0].data_ptr(), H * D, x[1].data_ptr(), G * D, x[2].data_ptr(), G * D, T, H, G, D, D,
+                                    1e4, t.tok_seq.data_ptr(), t.tok_pos.data_ptr(), t.table.data_ptr(), 2, cache[0].data_ptr(),
+                                    cache[1].data_ptr(), abi, q.data_ptr(), st) == 0
+        assert L.rtd_attention_paged(h.handle, q.data_ptr(), T, H, G, D, 0.125, t.tok_seq.data_ptr(), t.tok_pos.data_ptr(),
+                                     t.table.data_ptr(), 2, max_ctx, cache[0].data_ptr(), cache[1].data_ptr(), abi, o.data_ptr(),
+                                     _lib.DT_F32, H * D, st) == 0
+        return cache, o
+
+    def tables(max_tokens):
+        t = kv4.BlockTables(3, 2, 5, max_tokens)
+        t.step(torch.tensor([2, 0, 1], dtype=torch.int32, device="cuda"))
+        return t
+
+    padded, whole = tables(T), tables(3)
+    assert padded.tok_seq.tolist() == [0, 0, 2, -1, -1, -1]
+    (cache, o), (want, o3) = run(padded, T), run(whole, 3)
+    for a, b in zip(cache, want):
+        assert torch.equal(a, b)
+        assert (a != 3.0).any() and (a == 3.0).sum() == a.numel() - 3 * G * D  # three tokens, and nothing else
+    assert torch.equal(o[:3], o3) and not o[3:].any()
+    padded.step(torch.tensor([33, 0, 1], dtype=torch.int32, device="cuda"))  # more than the table holds: refused
+    with pytest.raises(ConfigError, match="paged cache"):
+        h.check_device_status()
+    assert (padded.tok_seq == -1).all()
+    cache, o = run(padded, T)
+    assert all((c == 3.0).all() for c in cache) and not o.any()
