@@ -283,8 +283,8 @@ rtd_status rtd_kv4_read(rtd_ctx* ctx, const int32_t* slots, int64_t n, int32_t n
  * takes queries and weights in 11 bits.  With 16-bit outputs prompt chunks (sequences with
  * 96 or more rows of queries x heads of the group, at head_dim 64 or 128, if they come to
  * 6144 or 4096 rows of queries x n_head in all) take queries, weights, keys and values
- * rounded to f16, where those beyond 65504 become infinite; a chunk's row that sees a NaN
- * group of V among the call's own tokens may be NaN in all dims of the head.
+ * rounded to f16; a chunk with keys or values beyond f16's 65504, or with a NaN group of V
+ * among the call's own tokens, is computed as above instead, as is any where o overlaps q.
  * o rows are ldo apart.  Long contexts are split over CTAs and joined in order, so equal
  * calls give equal bits.  A ctx_len outside 0 .. max_ctx counts as 0; a sequence with offsets
  * outside the T rows or with more than max_q queries is left alone; rows that read a block

@@ -828,11 +828,14 @@ rtd_status rtd_attention_kv4(rtd_ctx* ctx, const void* q, uint32_t q_dtype, int6
     return fail(ctx, RTD_ERR_SHAPE, "%s: max_ctx %d outside the block table (%d blocks, at most %d)", who, max_ctx, max_blocks,
                 INT32_MAX / 32);
   if (max_q <= 0) return fail(ctx, RTD_ERR_SHAPE, "%s: max_q %d", who, max_q);
+  const size_t parts = rtd::kv4_attention_ws_bytes(ctx->sm_count);
+  if (parts > ctx->ws_bytes)
+    return fail(ctx, RTD_ERR_WORKSPACE, "%s: the partial states do not fit the context workspace", who);
+  int* redo = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ctx->ws) + parts);
+  const int64_t redo_words = (int64_t)((ctx->ws_bytes - parts) / sizeof(int));
   rtd::Kv4Attention c{q, (int)q_dtype, ldq, T, n_head, n_kv, head_dim, scale, q_start, ctx_len, S, block_table,
                       max_blocks, max_q, max_ctx, static_cast<const uint8_t*>(pages), num_blocks, o, (int)o_dtype, ldo,
-                      ctx->ws, ctx->attn_count, ctx->status, ctx->sm_count, (cudaStream_t)stream};
-  if (rtd::kv4_attention_ws_bytes(ctx->sm_count) > ctx->ws_bytes)
-    return fail(ctx, RTD_ERR_WORKSPACE, "%s: the partial states do not fit the context workspace", who);
+                      ctx->ws, redo, redo_words, ctx->attn_count, ctx->status, ctx->sm_count, (cudaStream_t)stream};
   DeviceGuard g(ctx->device);
   if (g.err != cudaSuccess) return cuda_fail(ctx, g.err, who);
   cudaError_t e = rtd::launch_kv4_attention(c);

@@ -189,6 +189,8 @@ struct Kv4Attention {
   int o_dtype;
   int64_t ldo;
   float* ws;          // partial states: kv4_attention_ws_bytes
+  int* redo;          // [redo_words]: the prompt chunks that f16 operands cannot serve
+  int64_t redo_words;
   unsigned* count;    // kv4_attention_count_bytes, zero between calls (a word's last user clears it)
   int* status;
   int sm_count;

@@ -598,7 +598,8 @@ struct Attn {
       bad |= nq > 0;
       ctx = 0;
     }
-    if (nq * G >= wide_rows) nq = 0;  // the wide kernel's, which leaves the telling to this one
+    // the wide kernel's, which leaves the telling to this one, unless it met values beyond f16
+    if (nq * G >= wide_rows && !__ldg(a.redo + s)) nq = 0;
     if (bad && tell) raise_status(a.status, kDevCache);
     return kUnitCost + (ctx + kTok - 1) / kTok;
   }
@@ -1339,12 +1340,18 @@ cudaError_t launch_kv4_attention(const Kv4Attention& c) {
   const int wide_o = c.ldo % (c.o_dtype == 0 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(c.o) % 16 == 0;
   Kv4AttnArgs a{c.q, c.q_dtype, wide, c.ldq, (int)c.T, c.n_head, c.n_kv, c.scale, c.q_start, c.ctx_len, c.S, c.block_table,
                 c.max_blocks, c.max_q, c.max_ctx, c.pages, c.num_blocks, c.o, c.o_dtype, wide_o,
-                c.ldo, INT32_MAX, c.head_dim == 128 ? kWideTotal128 : kWideTotal64, kUnitCost + std::min(kWholePages, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
+                c.ldo, INT32_MAX, c.head_dim == 128 ? kWideTotal128 : kWideTotal64, c.redo, kUnitCost + std::min(kWholePages, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
   const bool exact = c.o_dtype != 2;  // bf16 rounds by 2^-9 what the other form rounds by 2^-11
   const int64_t rows = (int64_t)c.max_q * (c.n_head / c.n_kv);
-  if (c.o_dtype != 0 && (c.head_dim == 64 || c.head_dim == 128) && rows >= kWideRows && c.T * c.n_head >= a.wide_total) {
+  // outputs written over the queries are the line kernel's: it may have to read a chunk's again
+  auto bytes = [&](int dt, int64_t ld) { return ((c.T - 1) * ld + (int64_t)c.n_head * c.head_dim) * (dt == 0 ? 4 : 2); };
+  const uintptr_t q0 = reinterpret_cast<uintptr_t>(c.q), o0 = reinterpret_cast<uintptr_t>(c.o);
+  const bool apart = q0 + bytes(c.q_dtype, c.ldq) <= o0 || o0 + bytes(c.o_dtype, c.ldo) <= q0;
+  if (c.o_dtype != 0 && (c.head_dim == 64 || c.head_dim == 128) && rows >= kWideRows && c.T * c.n_head >= a.wide_total &&
+      apart && c.S <= c.redo_words) {
     a.wide_rows = kWideRows;
-    cudaError_t e = launch_kv4_wide(a, c.head_dim, c.stream);
+    cudaError_t e = cudaMemsetAsync(c.redo, 0, (size_t)c.S * sizeof(int), c.stream);
+    if (e == cudaSuccess) e = launch_kv4_wide(a, c.head_dim, c.stream);
     if (e != cudaSuccess) return e;  // what follows is for the others, if any
   }
   switch (c.head_dim / 32) {

@@ -93,6 +93,7 @@ struct Kv4AttnArgs {
   int64_t ldo;
   int wide_rows;    // sequences with at least so many rows (queries x G) are the wide kernel's,
   int64_t wide_total;  // if all of these have so many (queries x n_head) together
+  int* redo;        // [S] raised by the wide kernel: sequences of its that are the line kernel's all the same
   int min_share;    // pages a CTA takes at least
   float* part;      // [CTA][2][8 (D + 2)]: the units begun before it, and left open by it
   unsigned* count;  // [CTA]: parts done of the unit it leaves open, zero between calls

@@ -18,8 +18,11 @@
 // The running maximum moves only when a row's sum of p = 2^(x - max) over a key tile passes
 // 2^15: until then every p is below that, and inside f16.  So the maximum is looked for, and O
 // rescaled, rarely, and the exponentials come straight from the scores.  P, K, V and the
-// queries (scaled by a power of two per row) are rounded to f16's 11 bits; values beyond its
-// 65504 become infinite.
+// queries (scaled by a power of two per row) are rounded to f16's 11 bits.
+//
+// Keys or values beyond its 65504 have no place in these tiles, and a NaN of V that only some
+// rows of a tile see would reach the others as 0 * NaN.  A decoding thread that meets either
+// raises the sequence's word in `redo`, and the line kernel, which follows, writes all its rows.
 //
 // Bound: per 128 x 64 scores 512 clocks of tensor cores (at head_dim 128) and as many of the
 // exponential unit; what they take is the chain S -> softmax -> P -> S of a row tile.
@@ -359,6 +362,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
     // Four warps take the even stages, four the odd ones; of four, two turn K and two V.
     const int dw = (warp - kSoftWarps) & 3, odd_stage = (warp - kSoftWarps) >> 2;
     bool ok = nt == 0 || wait(q_full, 0);  // the queries have left
+    // the largest code's value, which is infinite where f16 is left (the least is f16 itself)
+    const __half2 fifteen = __float2half2_rn(15.0f);
+    __half2 largest = __float2half2_rn(0.0f);
+    bool redo = false;
     for (int j = 0; j < nt && ok; ++j) {
       const int buf = j % kBuf;
       if (j >= kBuf) ok = wait(kv_empty + buf, (uint32_t)((j / kBuf - 1) & 1));
@@ -381,14 +388,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
             const uint32_t page = raw + (kt >> 4) * PB;
             const bool there = key + kt < most;
             const int row = q * kStageKeys + kt;
-            // A NaN of V that some rows of the tile do not see would reach them as 0 * NaN.  From
-            // the first row's position on it goes into the key instead, whose score only the
-            // rows that see it take.
-            bool poison = false;
-            if (key + kStageKeys > least && there && key + kt >= least) {
-#pragma unroll
-              for (int g = 0; g < NG; ++g) poison |= (lds32(page + 18 * D + (t * NG + g) * 4) & 0x7c00u) == 0x7c00u;
-            }
             uint32_t w[4] = {}, h[4] = {};
             if (there) {
               const uint32_t at = page + t * (D / 2) + ki * NG * 4, head = page + 8 * D + t * NG * 4;
@@ -406,11 +405,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
               const __half2 d = __low2half2(as_h2(h[g])), m = __high2half2(as_h2(h[g]));
-              uint32_t v0 = as_u32(__hfma2(code_pair<false>(w[g]), d, m));
-              if (poison) v0 = 0x7fff7fffu;
+              largest = __hmax2(largest, __hfma2(fifteen, d, m));
               const int k = 32 * g + 8 * ki;
-              sts128(sm32 + P::offK + buf * P::kTile + (k >> 6) * (kKeys * 128) + sw_off(row, k & 63), v0,
-                     as_u32(__hfma2(code_pair<true>(w[g]), d, m)), as_u32(__hfma2(code_pair<false>(w[g] >> 8), d, m)),
+              sts128(sm32 + P::offK + buf * P::kTile + (k >> 6) * (kKeys * 128) + sw_off(row, k & 63),
+                     as_u32(__hfma2(code_pair<false>(w[g]), d, m)), as_u32(__hfma2(code_pair<true>(w[g]), d, m)), as_u32(__hfma2(code_pair<false>(w[g] >> 8), d, m)),
                      as_u32(__hfma2(code_pair<true>(w[g] >> 8), d, m)));
             }
           }
@@ -443,7 +441,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
             for (int e = 0; e < 8; ++e)
               if (key + 16 * (oct >> 1) + t0 + (e ^ swap) >= most) w[e] = h[e][0] = h[e][1] = 0;
           }
-          const bool diag = key + kStageKeys > least;
+          if (key + kStageKeys > least) {  // NaN that some rows do not see
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              redo |= key + 16 * (oct >> 1) + t0 + (e ^ swap) >= least &&
+                      ((h[e][0] & 0x7c00u) == 0x7c00u || (h[e][1] & 0x7c00u) == 0x7c00u);
+          }
           const int k = q * kStageKeys + 8 * oct;
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
@@ -452,20 +455,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
             for (int e = 0; e < 4; ++e) {
               const uint32_t x = prmt(w[2 * e], w[2 * e + 1], g ? high : low);
               const __half2 d = as_h2(prmt(h[2 * e][g], h[2 * e + 1][g], low)), m = as_h2(prmt(h[2 * e][g], h[2 * e + 1][g], high));
+              largest = __hmax2(largest, __hfma2(fifteen, d, m));
               out[0][e] = as_u32(__hfma2(code_pair<false>(x), d, m));
               out[1][e] = as_u32(__hfma2(code_pair<true>(x), d, m));
               out[2][e] = as_u32(__hfma2(code_pair<false>(x >> 8), d, m));
               out[3][e] = as_u32(__hfma2(code_pair<true>(x >> 8), d, m));
-              if (diag) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                  const int tok = b ^ swap;  // the half it lies in
-                  if (key + 16 * (oct >> 1) + t0 + 2 * e + tok >= least && (h[2 * e + b][g] & 0x7c00u) == 0x7c00u) {
-#pragma unroll
-                    for (int p = 0; p < 4; ++p) out[p][e] &= tok ? 0x0000ffffu : 0xffff0000u;
-                  }
-                }
-              }
             }
 #pragma unroll
             for (int p = 0; p < 4; ++p)
@@ -478,6 +472,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_wide_kernel(const Kv4Attn
       fence_async_shared();
       mbar_arrive(kv_full + buf);
     }
+    redo |= __hisinf(__low2half(largest)) || __hisinf(__high2half(largest));
+    if (redo) a.redo[s] = 1;
   } else {
     // ------------------------------------------------------------ softmax, a thread a row
     regs_up<kSoftRegs>();
