@@ -767,7 +767,7 @@ struct Attn {
     // ---- sums of p times what a group's codes add to: its minimum, or, about code 8, the
     // middle m + 8 d.  The middles lie around zero, where the sums of the minima and of the
     // steps would each grow and then cancel; column g takes the middle as f16, column 4 + g
-    // the rest (two-sum).  On a second attempt, whose 8 d may pass f16's range, an eighth.
+    // the rest (two-sum).  On a second attempt, whose m + 8 d may pass f16's range, a 16th.
     const uint32_t vh = page + 18 * D;
     {
       const int g = min(r & 3, NG - 1);
@@ -778,7 +778,7 @@ struct Attn {
         const uint32_t w0 = lds(at + 32 * NG * u), w1 = lds(at + 32 * NG * u + 16 * NG);
         b[u] = prmt(w0, w1, 0x7632u);
         if constexpr (EXACT) {
-          const __half2 s8 = __float2half2_rn(attempt ? 1.0f : 8.0f), s1 = __float2half2_rn(attempt ? 0.125f : 1.0f);
+          const __half2 s8 = __float2half2_rn(attempt ? 0.5f : 8.0f), s1 = __float2half2_rn(attempt ? 0.0625f : 1.0f);
           const __half2 x = __hmul2_rn(as_h2(prmt(w0, w1, 0x5410u)), s8), y = __hmul2_rn(as_h2(b[u]), s1);
           const __half2 sum = __hadd2_rn(x, y), v = __hsub2_rn(sum, x);
           const __half2 rest = __hadd2_rn(__hsub2_rn(x, __hsub2_rn(sum, v)), __hsub2_rn(y, v));
@@ -1017,7 +1017,7 @@ struct Attn {
       if (attempt) {
         if constexpr (EXACT)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) z[c] *= 8.0f;
+          for (int c = 0; c < 4; ++c) z[c] *= 16.0f;
         break;
       }
       if (mine == 0) break;

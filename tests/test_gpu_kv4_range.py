@@ -107,3 +107,17 @@ def test_outputs_over_the_queries(D):
             x = dev(q).to(dt)
             rows = x.float().cpu().numpy()
             close(c, rows, run_attention(c, x, [N], out=x), dt)
+
+
+@pytest.mark.parametrize("D,low,high", [(64, 60000, 1e6), (128, -65000, 9e5), (32, 0, 65504 * 15), (96, 65504, 65504 * 16)])
+def test_groups_whose_middle_is_beyond_f16(D, low, high):
+    # step and minimum are f16, minimum + 8 steps is not: read with a 16th of the middle
+    c = Case([70, 20], 2, D, seed=D)
+    v = np.concatenate(c.V).astype(np.float32)
+    v[33, 1, :32] = np.linspace(low, high, 32)
+    c.write(np.concatenate(c.K).astype(np.float32), v, np.concatenate(c.slots))
+    assert np.isfinite(c.V[0]).all() and c.V[0].max() > 8e5
+    q = np.random.default_rng(4).normal(0, 1, (5, 8, D)).astype(np.float32)
+    got = run_attention(c, dev(q), [4, 1]).cpu().numpy()
+    want, tol = c.want(q.astype(np.float64), [4, 1], 1 / math.sqrt(D))
+    assert np.all(np.abs(got - want) <= tol)
