@@ -561,13 +561,13 @@ struct Attn {
   static constexpr int kPart = kRows * (D + 2);
   static constexpr int kJoinBytes = kAttnWarps * kState * 4;
   static constexpr int kCols = EXACT ? 2 : 4;  // sums of a fragment: of both row halves, or as the MMA has them
-  static constexpr int kSmem = kAttnWarps * kStages * PB + kJoinBytes + NG * 1024;
+  static constexpr int kSmem = kAttnWarps * kStages * PB + kJoinBytes + NG * 1024 + 4 * kAttnWarps;
   const Kv4AttnArgs& a;
   uint8_t* ring;      // this warp's pages
   uint32_t ring32;
   uint64_t* bars;     // and their barriers
   float* join;        // the warps' states
-  uint32_t qfrag;     // this lane's query fragments, [group][k step][lane][16 bytes]
+  uint32_t qfrag;     // this lane's query fragments, [group][k step][lane][16 bytes]; behind them the warps' lifts
   int G, lane, warp;
   int wide_rows = INT32_MAX;    // a.wide_rows where the chunks are many enough
   unsigned get = 0, phase = 0;  // the ring's next page to use, and its parity
@@ -762,12 +762,12 @@ struct Attn {
 
   // O += (p d) C and the header sums z of a page, p = ph + pl of pairs of tokens (i, i + 4) and
   // (i + 8, i + 12).
-  __device__ void values(uint32_t page, int attempt, int r, int qi, const uint32_t (&ph)[2], const uint32_t (&pl)[2],
+  __device__ void values(uint32_t page, bool large, int r, int qi, const uint32_t (&ph)[2], const uint32_t (&pl)[2],
                          float (&o)[NG][4][kCols], float (&z)[4]) const {
     // ---- sums of p times what a group's codes add to: its minimum, or, about code 8, the
     // middle m + 8 d.  The middles lie around zero, where the sums of the minima and of the
     // steps would each grow and then cancel; column g takes the middle as f16, column 4 + g
-    // the rest (two-sum).  On a second attempt, whose m + 8 d may pass f16's range, a 16th.
+    // the rest (two-sum).  Where m + 8 d may pass f16's range (`large`), a 16th.
     const uint32_t vh = page + 18 * D;
     {
       const int g = min(r & 3, NG - 1);
@@ -778,7 +778,7 @@ struct Attn {
         const uint32_t w0 = lds(at + 32 * NG * u), w1 = lds(at + 32 * NG * u + 16 * NG);
         b[u] = prmt(w0, w1, 0x7632u);
         if constexpr (EXACT) {
-          const __half2 s8 = __float2half2_rn(attempt ? 0.5f : 8.0f), s1 = __float2half2_rn(attempt ? 0.0625f : 1.0f);
+          const __half2 s8 = __float2half2_rn(large ? 0.5f : 8.0f), s1 = __float2half2_rn(large ? 0.0625f : 1.0f);
           const __half2 x = __hmul2_rn(as_h2(prmt(w0, w1, 0x5410u)), s8), y = __hmul2_rn(as_h2(b[u]), s1);
           const __half2 sum = __hadd2_rn(x, y), v = __hsub2_rn(sum, x);
           const __half2 rest = __hadd2_rn(__hsub2_rn(x, __hsub2_rn(sum, v)), __hsub2_rn(y, v));
@@ -807,12 +807,14 @@ struct Attn {
         if constexpr (NG & 1) vw[c][NG / 2] = lds_half(vr + ((NG - 1) * 8 + r) * 2);
       }
     }
+    const __half2 lift = as_h2(EXACT ? lds(lift_at()) : 0u);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       uint32_t hi[2], lo[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const __half2 d = as_h2(prmt(vd[2 * u][g], vd[2 * u + 1][g], 0x5410u));
+        __half2 d = as_h2(prmt(vd[2 * u][g], vd[2 * u + 1][g], 0x5410u));
+        if constexpr (EXACT) d = __hmul2(d, lift);
         const __half2 p = as_h2(ph[u]), h = __hmul2(p, d);
         hi[u] = as_u32(h);
         lo[u] = EXACT ? as_u32(__hfma2(as_h2(pl[u]), d, __hfma2(p, d, __hneg2(h)))) : 0u;
@@ -825,6 +827,29 @@ struct Attn {
       add(o[g][3], hi, lo, codes<EXACT, 8, true>(b0 >> 8), codes<EXACT, 8, true>(b1 >> 8));
     }
   }
+
+  // Small steps are lifted by a power of two, at most 2^15: the rest of p d lies on f16's grid of
+  // 2^-24, which with p d of 2^-7 was 4e-6 of it.  The largest step of a warp's first page (the
+  // keys that any row sees) goes to 2^-4 .. 2^-3, and later ones may be 256 times as large.
+  __device__ int lift_of(uint32_t vh, int keys) const {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < (16 * NG + 31) / 32; ++i) {
+      const int at = 32 * i + lane;
+      const uint32_t d = at < NG * min(kTok, keys) ? lds(vh + 4 * at) & 0x7fffu : 0u;
+      if (d < 0x7c00u) most = max(most, d);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    return most ? max(0, min(15, -4 - ilogbf(f16_bits_to_f32(most)))) : 0;
+  }
+  // Kept in shared memory, an f16 pair of 2^lift: the loop over the pages has no register left.
+  __device__ uint32_t lift_at() const { return qfrag - 16 * lane + NG * 1024 + 4 * warp; }
+  __device__ void set_lift(int by) const {
+    __syncwarp();
+    if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(lift_at()), "r"(0x3c003c00u + by * 0x04000400u) : "memory");
+    __syncwarp();
+  }
+  __device__ int lift_now() const { return (int)(lds(lift_at()) >> 26) - 15; }
 
   // A page with keys that some row does not see: such keys weigh nothing, whatever they hold,
   // so V headers that are not finite are zeroed, since 0 * NaN would reach every row of the
@@ -944,10 +969,11 @@ struct Attn {
 
     const int kt = ((r & 1) << 2) | (r >> 1);  // token of S column r: columns 2 i, 2 i + 1 are tokens i, i + 4
     // p = 2^(x - max + headroom) right after a maximum is set, which stays until a score
-    // would pass 2^growth; if p d left f16's range after all (a step above 16), the pages
-    // are read once more with p at most 1
+    // would pass 2^growth; if p d left f16's range after all, the pages are read once more
+    // without the lift and, if that was not it (a step above 16), with p at most 1
+    if (EXACT) set_lift(0);
     for (int attempt = 0;; ++attempt) {
-      const float headroom = attempt ? 0.0f : 8.0f, growth = attempt ? 0.0f : 12.0f;
+      const float headroom = attempt == 2 ? 0.0f : 8.0f, growth = attempt == 2 ? 0.0f : 12.0f;
       M = -1e30f;
       l = 0.0f;
 #pragma unroll
@@ -1010,11 +1036,13 @@ struct Attn {
             pl[u] = as_u32(__floats2half2_rn(p0 - f.x, p1 - f.y));
           }
         }
-        values(page, attempt, r, qi, ph, pl, o, z);
+        if constexpr (EXACT)
+          if (j == 0 && attempt == 0) set_lift(lift_of(page + 18 * D, most - key));
+        values(page, attempt == 2, r, qi, ph, pl, o, z);
         __syncwarp();
         if (j & 1) issue(sg, j + kStages - 1);  // the two pages just used
       }
-      if (attempt) {
+      if (attempt == 2) {
         if constexpr (EXACT)
 #pragma unroll
           for (int c = 0; c < 4; ++c) z[c] *= 16.0f;
@@ -1031,6 +1059,8 @@ struct Attn {
 #pragma unroll
       for (int c = 0; c < 4; ++c) probe = fmaf(z[c], 0.0f, probe);
       if (!__any_sync(0xffffffffu, probe != 0.0f)) break;  // NaN where anything was not finite
+      if (!EXACT || lift_now() == 0) attempt = 1;
+      if (EXACT) set_lift(0);
       // from the start once more: the ring is empty, and an odd number of pages may have used it
       sg.ids = load_ids(sg, 0);
       for (int j = 0; j < kStages; j += 2) issue(sg, j);
@@ -1051,6 +1081,7 @@ struct Attn {
     }
     {
       float* out = join + warp * kState + r * kPitch + 8 * qi;
+      const float down = EXACT ? pow2(-lift_now()) : 1.0f;
       const float z0 = z[0] + z[2], z1 = z[1] + z[3];  // quad lanes 0, 1: middles or minima; 2, 3: their rests
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -1061,7 +1092,7 @@ struct Attn {
         float v[8];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          const float f = (EXACT ? 1.0f : 16777216.0f) * ((p & 1) ? 0.0625f : 1.0f);  // the odd nibbles' 16
+          const float f = (EXACT ? down : 16777216.0f) * ((p & 1) ? 0.0625f : 1.0f);  // the odd nibbles' 16
           v[p] = fmaf(o[g][p][0] + (EXACT ? 0.0f : o[g][p][kCols - 2]), f, zz);
           v[4 + p] = fmaf(o[g][p][1] + (EXACT ? 0.0f : o[g][p][kCols - 1]), f, zz);
         }
