@@ -290,7 +290,7 @@ rtd_status rtd_kv4_read(rtd_ctx* ctx, const int32_t* slots, int64_t n, int32_t n
  * outside the T rows or with more than max_q queries is left alone; rows that read a block
  * outside the pool become NaN: each with RTD_ERR_CACHE in the status word.  The parts lie in the
  * context's workspace and their counts in the context: calls of one context must not overlap
- * on the GPU. */
+ * on the GPU.  Where they do, the outputs of those calls mean nothing; later calls are right. */
 rtd_status rtd_attention_kv4(rtd_ctx* ctx, const void* q, uint32_t q_dtype, int64_t ldq, int64_t T, int32_t n_head,
                              int32_t n_kv, int32_t head_dim, float scale, const int32_t* q_start,
                              const int32_t* ctx_len, int32_t S, const int32_t* block_table, int32_t max_blocks,

@@ -28,7 +28,7 @@ struct rtd_ctx {
   int* status = nullptr;
   // rtd_qlinear_argmax's epilogue state: [4] packed keys and a CTA count, zero between calls
   unsigned long long* amax = nullptr;
-  // rtd_attention_kv4's CTAs-done words, zero between calls
+  // rtd_attention_kv4's arrival words, whole multiples of 2^20 between calls
   unsigned* attn_count = nullptr;
   std::string err;
 };

@@ -191,7 +191,7 @@ struct Kv4Attention {
   float* ws;          // partial states: kv4_attention_ws_bytes
   int* redo;          // [redo_words]: the prompt chunks that f16 operands cannot serve
   int64_t redo_words;
-  unsigned* count;    // kv4_attention_count_bytes, zero between calls (a word's last user clears it)
+  unsigned* count;    // kv4_attention_count_bytes, zero at first
   int* status;
   int sm_count;
   cudaStream_t stream;

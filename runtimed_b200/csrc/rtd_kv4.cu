@@ -460,6 +460,7 @@ constexpr int kStages = 4;  // even: pages are asked for in pairs (six do not fi
 constexpr int kRows = 8;
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 512;
+constexpr unsigned kArrive = 1u << 20;  // more than CTAs
 // Sequences with so many rows (queries x heads of the group) are prompt chunks: with 96 rows
 // the chunk kernel's 256-row tile is as fast as 12 tiles of 8 here if other chunks fill the GPU
 // (16 sequences of 2000, 64/8 heads of 128: 64 rows 66 us there, 111 here; 32 rows 66 and 63).
@@ -1159,7 +1160,9 @@ struct Attn {
 
   // The units that this CTA shares (the one begun before it, the one it leaves open): the last
   // CTA of a unit to come here joins its parts, in CTA order.  Once, at the end of the CTA's
-  // stretch: the fence and the atomics cost 3 us a time.
+  // stretch: the fence and the atomics cost 3 us a time.  A unit's CTAs add a whole kArrive in all
+  // to its word, which only the last to arrive fills up.  Nobody clears it: calls that overlapped
+  // spoil one another's parts, but leave whole multiples behind, and later calls count as ever.
   __device__ void join_parts(Open* left) {
     const int tid = threadIdx.x;
     if (tid < 2) {
@@ -1167,8 +1170,8 @@ struct Attn {
       u.last = 0;
       if (u.c0 >= 0) {
         __threadfence();
-        u.last = atomicAdd(a.count + u.c0, 1u) == (unsigned)(u.c1 - u.c0);
-        if (u.last) a.count[u.c0] = 0;
+        const unsigned add = (int)blockIdx.x == u.c0 ? kArrive - (unsigned)(u.c1 - u.c0) : 1u;
+        u.last = (atomicAdd(a.count + u.c0, add) + add) % kArrive == 0;
         __threadfence();
       }
     }

@@ -96,7 +96,7 @@ struct Kv4AttnArgs {
   int* redo;        // [S] raised by the wide kernel: sequences of its that are the line kernel's all the same
   int min_share;    // pages a CTA takes at least
   float* part;      // [CTA][2][8 (D + 2)]: the units begun before it, and left open by it
-  unsigned* count;  // [CTA]: parts done of the unit it leaves open, zero between calls
+  unsigned* count;  // [CTA]: arrivals at the unit it leaves open, whole kArrive between calls
   int* status;
 };
 
