@@ -519,7 +519,9 @@ class Qwen2Model:
         blocks from the device's free stack), the layers run over the tokens it lists, and
         rtd_sample puts the next ids where the next step reads them; with `graph` the step
         is captured once and replayed.  The random numbers come from torch's generator
-        seeded with `seed`, one per sequence and step, so equal calls give equal ids."""
+        seeded with `seed`, one per sequence and step, so equal calls give equal ids.
+        What the device reported on the way (``Context.check_device_status``) is raised at the
+        end."""
         from . import kv4, sampling
 
         b, cache = len(prompts), self.cache
@@ -546,6 +548,7 @@ class Qwen2Model:
         sampling.sample(last, now, *filters, out=ids)
         out[0].copy_(ids)
         if steps == 1:
+            self.ctx.check_device_status()
             return out.t().contiguous()
         tables = kv4.BlockTables.from_cache(cache, b)
         grow = torch.zeros((cache.max_seqs,), dtype=torch.int32, device=dev)
@@ -575,6 +578,7 @@ class Qwen2Model:
             replay()
             out[i].copy_(ids)
         tables.into(cache)
+        self.ctx.check_device_status()  # the ids of a step that was refused, or gave up a wait, are none
         return out.t().contiguous()
 
     def sample(self, logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,

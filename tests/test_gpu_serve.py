@@ -215,3 +215,28 @@ def test_padded_rows_of_a_plan_leave_the_16_and_32_bit_caches_alone(kv):
     assert (padded.tok_seq == -1).all()
     cache, o = run(padded, T)
     assert all((c == 3.0).all() for c in cache) and not o.any()
+
+
+@pytest.mark.parametrize("kv", ["q4", torch.float16])
+@pytest.mark.parametrize("graph", [True, False])
+def test_generate_batch_raises_what_a_step_reported(gguf, kv, graph, monkeypatch):
+    # a free stack that is empty on the device: the second step wants a block for each sequence
+    from runtimed_b200 import kv4
+    from runtimed_b200.errors import ConfigError
+
+    take_over = kv4.BlockTables.from_cache.__func__
+
+    def none_free(cls, cache, max_tokens):
+        t = take_over(cls, cache, max_tokens)
+        t.free_count.zero_()
+        return t
+
+    m = model(gguf, kv)
+    monkeypatch.setattr(kv4.BlockTables, "from_cache", classmethod(none_free))
+    with pytest.raises(ConfigError, match="paged cache"):
+        m.generate_batch(prompts(16, 32), 3, graph=graph)
+    assert m.cache.lengths == {0: 16, 1: 32}
+    monkeypatch.undo()
+    m.ctx.check_device_status()  # told once
+    fresh = model(gguf, kv)
+    assert torch.equal(fresh.generate_batch(prompts(16, 32), 3, graph=graph), model(gguf, kv).generate_batch(prompts(16, 32), 3))
