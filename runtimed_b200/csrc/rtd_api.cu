@@ -156,12 +156,23 @@ rtd_status rtd_init(int device, rtd_ctx** out) {
     return fail(nullptr, RTD_ERR_CUDA, "rtd_init: cudaSetDevice: %s", cudaGetErrorString(g.err));
   }
   cudaDeviceGetAttribute(&c->sm_count, cudaDevAttrMultiProcessorCount, device);
-  if ((e = cudaMalloc(&c->ws, kWorkspaceBytes)) != cudaSuccess ||
-      (e = cudaMalloc(&c->status, sizeof(int))) != cudaSuccess ||
-      (e = cudaMemset(c->status, 0, sizeof(int))) != cudaSuccess ||
-      (e = cudaMalloc(&c->amax, kAmaxBytes)) != cudaSuccess || (e = cudaMemset(c->amax, 0, kAmaxBytes)) != cudaSuccess ||
-      (e = cudaMalloc(&c->attn_count, rtd::kv4_attention_count_bytes(c->sm_count))) != cudaSuccess ||
-      (e = cudaMemset(c->attn_count, 0, rtd::kv4_attention_count_bytes(c->sm_count))) != cudaSuccess) {
+  // The first call on a device may lie in a stream capture: allocations are then allowed in the
+  // relaxed mode only, and the clearing goes to a stream of its own (the legacy stream would join
+  // the capture), which is waited for, since callers' streams need not wait for another.
+  const size_t count_bytes = rtd::kv4_attention_count_bytes(c->sm_count);
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  cudaStream_t st = nullptr;
+  if ((e = cudaMalloc(&c->ws, kWorkspaceBytes)) == cudaSuccess && (e = cudaMalloc(&c->status, sizeof(int))) == cudaSuccess &&
+      (e = cudaMalloc(&c->amax, kAmaxBytes)) == cudaSuccess && (e = cudaMalloc(&c->attn_count, count_bytes)) == cudaSuccess &&
+      (e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking)) == cudaSuccess &&
+      (e = cudaMemsetAsync(c->status, 0, sizeof(int), st)) == cudaSuccess &&
+      (e = cudaMemsetAsync(c->amax, 0, kAmaxBytes, st)) == cudaSuccess &&
+      (e = cudaMemsetAsync(c->attn_count, 0, count_bytes, st)) == cudaSuccess)
+    e = cudaStreamSynchronize(st);
+  if (st) cudaStreamDestroy(st);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) {
     cudaFree(c->ws);
     cudaFree(c->status);
     cudaFree(c->amax);
