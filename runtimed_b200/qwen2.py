@@ -367,7 +367,8 @@ class Qwen2Model:
             fq = self.fused.get((i, "qkv"))
             if fq is not None:  # q | k | v from one launch: column slices of one output
                 qkv = self._lin(n, cfg.hidden, T, fq[0], fq[1])
-                q, k, v = qkv.split(fq[2], 1)
+                if self.cache.q4:
+                    q, k, v = qkv.split(fq[2], 1)
                 w = qkv.shape[1]
                 qp, kp = qkv.data_ptr(), qkv.data_ptr() + 4 * fq[2][0]
                 vp = kp + 4 * fq[2][1]
