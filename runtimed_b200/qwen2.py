@@ -529,12 +529,13 @@ class Qwen2Model:
         if not 0 < b <= cache.max_seqs or steps < 1 or not all(len(p) for p in prompts):
             raise ConfigError(f"{b} prompts for {cache.max_seqs} sequences, {steps} steps (a prompt has a token at least)")
         longest = max(len(p) for p in prompts) + steps
+        need = sum(-(-(len(p) + steps) // KV_BLOCK) for p in prompts)
+        free = len(cache._free) + sum(len(cache._blocks.get(s, ())) for s in range(b))  # theirs are given back
+        if -(-longest // KV_BLOCK) > cache.max_blocks or need > free:
+            raise ConfigError(f"KV cache: {need} blocks for {longest} tokens of a sequence, {free} free, "
+                              f"{cache.max_blocks} a sequence")
         for s in range(b):
             cache.release(s)
-        need = sum(-(-(len(p) + steps) // KV_BLOCK) for p in prompts)
-        if -(-longest // KV_BLOCK) > cache.max_blocks or need > len(cache._free):
-            raise ConfigError(f"KV cache: {need} blocks for {longest} tokens of a sequence, {len(cache._free)} free, "
-                              f"{cache.max_blocks} a sequence")
         dev, f32 = self.device, torch.float32
         gen = torch.Generator(device=dev)
         gen.manual_seed(seed)

@@ -240,3 +240,17 @@ def test_generate_batch_raises_what_a_step_reported(gguf, kv, graph, monkeypatch
     m.ctx.check_device_status()  # told once
     fresh = model(gguf, kv)
     assert torch.equal(fresh.generate_batch(prompts(16, 32), 3, graph=graph), model(gguf, kv).generate_batch(prompts(16, 32), 3))
+
+
+def test_a_refused_generate_batch_leaves_its_sequences(gguf):
+    from runtimed_b200.errors import ConfigError
+
+    m = model(gguf, "q4", kv_blocks=6)
+    p = prompts(40)[0]
+    m.forward(p, 0, seq=0)
+    kept = [x.clone() for x in m.cache.values(1, 0)]
+    with pytest.raises(ConfigError):
+        m.generate_batch(prompts(90), 20)
+    assert m.cache.lengths == {0: 40} and all(torch.equal(a, b) for a, b in zip(kept, m.cache.values(1, 0)))
+    assert m.generate_batch(prompts(70), 20).shape == (1, 20)  # six blocks, three of them sequence 0's own
+    assert m.cache.lengths == {0: 89}
