@@ -281,10 +281,12 @@ rtd_status rtd_kv4_read(rtd_ctx* ctx, const int32_t* slots, int64_t n, int32_t n
  * Accuracy: an f32 or f16 output is that of exact codes with queries and weights in 22 bits
  * or more and 32-bit sums, about 5e-7 of the result before its own rounding; a bf16 output
  * takes queries and weights in 11 bits.  With 16-bit outputs prompt chunks (sequences with
- * 96 or more rows of queries x heads of the group, at head_dim 64 or 128, if they come to
- * 6144 or 4096 rows of queries x n_head in all) take queries, weights, keys and values
- * rounded to f16; a chunk with keys or values beyond f16's 65504, or with a NaN group of V
- * among the call's own tokens, is computed as above instead, as is any where o overlaps q.
+ * 64 or more rows of queries x heads of the group, 96 with f16 outputs, at head_dim 64 or 128,
+ * if they come to 6144 or 4096 rows of queries x n_head in all) take queries, weights, keys
+ * and values rounded to f16: f16 outputs are then about 6e-4 of 64 bits, where those above are
+ * 2e-4 (their own rounding).  A chunk with keys or values beyond f16's 65504, or with a NaN
+ * group of V among the call's own tokens, is computed as above instead, as is any where o
+ * overlaps q.
  * o rows are ldo apart.  Long contexts are split over CTAs and joined in order, so equal
  * calls give equal bits.  A ctx_len outside 0 .. max_ctx counts as 0; a sequence with offsets
  * outside the T rows or with more than max_q queries is left alone; rows that read a block

@@ -461,10 +461,12 @@ constexpr int kRows = 8;
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 512;
 constexpr unsigned kArrive = 1u << 20;  // more than CTAs
-// Sequences with so many rows (queries x heads of the group) are prompt chunks: with 96 rows
-// the chunk kernel's 256-row tile is as fast as 12 tiles of 8 here if other chunks fill the GPU
-// (16 sequences of 2000, 64/8 heads of 128: 64 rows 66 us there, 111 here; 32 rows 66 and 63).
-constexpr int kWideRows = 96;
+// Sequences with so many rows (queries x heads of the group) are prompt chunks.  With other chunks
+// filling the GPU (16 sequences of 2000, 64/8 heads of 128) 64 rows take 83 us there, 121 here with
+// bf16 outputs and 137 with f16, 48 rows 83 against 94 and 109; of 64 dims (64 sequences of 1000)
+// 64 rows 150 against 154 and 180, 48 rows 150 against 118 and 139.  f16 outputs, whose queries and
+// weights have 22 bits here and 11 there, stay longer: 80 rows take 83 us there, 165 here.
+constexpr int kWideRowsBf16 = 64, kWideRowsF16 = 96;
 // A chunk tile takes its time however few there are, so all chunks together need so many rows
 // (queries x n_head).  One sequence of 4000, 64/8 heads: of 128, 2048 rows take 98 us there and
 // 58 here, 4096 98 and 103; of 64, 4096 take 85 and 66, 8192 85 and 121.
@@ -1377,13 +1379,14 @@ cudaError_t launch_kv4_attention(const Kv4Attention& c) {
                 c.ldo, INT32_MAX, c.head_dim == 128 ? kWideTotal128 : kWideTotal64, c.redo, kUnitCost + std::min(kWholePages, (c.max_ctx + kTok - 1) / kTok), c.ws, c.count, c.status};
   const bool exact = c.o_dtype != 2;  // bf16 rounds by 2^-9 what the other form rounds by 2^-11
   const int64_t rows = (int64_t)c.max_q * (c.n_head / c.n_kv);
+  const int wide_rows = c.o_dtype == 2 ? kWideRowsBf16 : kWideRowsF16;
   // outputs written over the queries are the line kernel's: it may have to read a chunk's again
   auto bytes = [&](int dt, int64_t ld) { return ((c.T - 1) * ld + (int64_t)c.n_head * c.head_dim) * (dt == 0 ? 4 : 2); };
   const uintptr_t q0 = reinterpret_cast<uintptr_t>(c.q), o0 = reinterpret_cast<uintptr_t>(c.o);
   const bool apart = q0 + bytes(c.q_dtype, c.ldq) <= o0 || o0 + bytes(c.o_dtype, c.ldo) <= q0;
-  if (c.o_dtype != 0 && (c.head_dim == 64 || c.head_dim == 128) && rows >= kWideRows && c.T * c.n_head >= a.wide_total &&
+  if (c.o_dtype != 0 && (c.head_dim == 64 || c.head_dim == 128) && rows >= wide_rows && c.T * c.n_head >= a.wide_total &&
       apart && c.S <= c.redo_words) {
-    a.wide_rows = kWideRows;
+    a.wide_rows = wide_rows;
     cudaError_t e = cudaMemsetAsync(c.redo, 0, (size_t)c.S * sizeof(int), c.stream);
     if (e == cudaSuccess) e = launch_kv4_wide(a, c.head_dim, c.stream);
     if (e != cudaSuccess) return e;  // what follows is for the others, if any

@@ -87,3 +87,20 @@ def test_values_that_grow_after_the_first_pages(first):
     v[300:] *= 30
     c.write(c.K[0].astype(np.float32), v, c.slots[0])
     check(c, [2], 8)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,new", [([4000], [130]), ([9000, 2500], [40, 70]), ([300] * 8, [12] * 8), ([700] * 12, [8] * 12)])
+def test_prompt_chunks(D, lens, new, out_dtype):
+    # Queries, keys, weights and values of f16's 11 bits, 2e-4 each on average: with keys about one,
+    # not zero, a score's two count 3e-4 each, 5e-4 in all, beside half a step of the output.
+    # f16 outputs of the other kernel (12 x 8 queries of 8 heads a group) come closer.
+    c = Case(lens, 8, D, seed=len(lens) + D)
+    q = np.random.default_rng(1).normal(0, 1, (sum(new), 64, D)).astype(np.float32)
+    got = run_attention(c, dev(q), new, out_dtype=out_dtype).double().cpu().numpy()
+    limit = 8e-4 if out_dtype == torch.float16 else 2.6e-3
+    at = 0
+    for s, want in enumerate(wanted(c, q.astype(np.float64), new)):
+        assert rel(got[at:at + new[s]] - want, want) <= limit, (s, rel(got[at:at + new[s]] - want, want))
+        at += new[s]
