@@ -162,7 +162,6 @@ PyObject* plan(PyObject* const* a, Py_ssize_t n) {
   void* lists[4] = {};
   int64_t tokens = 0;
   at::Tensor fresh[4];
-  PyObject* result = nullptr;
   if (a[6] != Py_None) {
     if (!PyTuple_Check(a[6]) || PyTuple_GET_SIZE(a[6]) != 4) config_error("out: (q_start, tok_seq, tok_pos, tok_slot) is wanted");
     static const char* names[4] = {"q_start", "tok_seq", "tok_pos", "tok_slot"};
@@ -172,7 +171,6 @@ PyObject* plan(PyObject* const* a, Py_ssize_t n) {
       lists[i] = dense(names[i], t, at::kInt, dev, {i ? tokens : s + 1});
     }
     if (tokens > INT32_MAX) config_error("plan: sizes beyond 32 bits");
-    result = Py_NewRef(a[6]);
   } else if (a[5] != Py_None) {
     tokens = integer("max_tokens", a[5]);
     if (tokens < 0) config_error("max_tokens: " + std::to_string(tokens));
@@ -189,11 +187,10 @@ PyObject* plan(PyObject* const* a, Py_ssize_t n) {
                                     static_cast<int32_t*>(lists[0]), static_cast<int32_t*>(lists[1]),
                                     static_cast<int32_t*>(lists[2]), static_cast<int32_t*>(lists[3]), (int32_t)tokens,
                                     stream(dev));
-  if (st != RTD_OK) Py_CLEAR(result);
   check(st, dev);
-  if (result) return result;
+  if (a[6] != Py_None) return Py_NewRef(a[6]);
   if (a[5] == Py_None) Py_RETURN_NONE;
-  result = PyTuple_New(4);
+  PyObject* result = PyTuple_New(4);
   for (int i = 0; result && i < 4; ++i) PyTuple_SET_ITEM(result, i, wrap(std::move(fresh[i])));
   return result;
 }
