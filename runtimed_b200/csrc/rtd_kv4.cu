@@ -204,11 +204,12 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
 // either half, asked for before the angles are formed.  Of the other heads a warp takes one
 // at a time, lane = dim within the group: the group's extremes come from two warp reductions
 // over order-mapped integers, whose ends also reveal infinities and NaN.
-// Bound: HBM.  2000 tokens of 64/8 heads of 128 in f32 move 161 MB, 25 us at the copy rate;
-// 44 us here, 59 with a lane per dim for the queries too (4-byte accesses).  The angles'
-// 64-bit sines hold up a CTA for 2 us, with four or five CTAs on an SM.
+// Bound: HBM.  2000 tokens of 64/8 heads of 128 in f32 move 150 MB, 23 us at the copy rate; 38 us
+// here (bf16 and f16, 109 MB, 17 us: 36).  The angles' 64-bit sines hold up a CTA for 2 us, with
+// four or five CTAs on an SM.  With a lane per dim for the queries too (4-byte accesses) append
+// and reader together took 59 us, 44 as they are.
 constexpr int kAppThreads = 256;
-constexpr int kAppQuads = 2;  // 44 us as above; 1: 47; 4: 51, since fewer CTAs fit
+constexpr int kAppQuads = 2;  // those 44 us; 1: 47; 4: 51, since fewer CTAs fit
 
 struct AppendArgs {
   const void* q;
@@ -444,16 +445,18 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const int* slots, int64_t
 // difference of two large ones.
 // Otherwise (bf16 outputs): the rows enter rounded to 11 bits and the nibble stays the
 // f16 subnormal c * 2^-24, which saves the addition; the tensor cores align a subnormal's
-// product as if its leading zeros counted, which costs 2e-5 of the output.  f16 outputs were
-// 5e-4 off in this form, where rounding them costs 2e-4.
+// product as if its leading zeros counted, which costs 2e-5 of the output.  bf16 outputs come out
+// 1.77e-3 off 64 bits, where their own rounding is 1.65e-3; f16 ones were 5e-4 off in this form,
+// where rounding them costs 2e-4.
 //
 // Bound: 64 sequences of up to 4096 tokens, 64 query heads on 8 (f32 outputs) read 240 MB,
 // 37 us at the copy rate; the kernel takes 97 us (2.5 TB/s), 3 sequences of up to 60000 in
-// bf16 (184 MB, 28 us) 69 us.  It is the instructions: a page costs a warp 450 with f32
-// outputs, and a scheduler with its three warps issues in half the cycles.  With the scores
-// left out an earlier version of 111 us took 80, with the values 85, with both 65.  Two CTAs
-// an SM with rings of eight pages and four with rings of three were no faster, nor was a loop
-// over page pairs; five stages cost 4 us with f32 outputs.
+// bf16 (184 MB, 28 us) 69 us, in f16 78.  Neither the bytes nor the issue slots (57 % of a
+// scheduler's cycles; 600 instructions a page) bound it but a page's chain scores -> softmax ->
+// values, which three warps a scheduler do not hide: fixed latencies, and the ALU (44 %) and
+// FMA (39 %) pipes in bursts.  Of an earlier version's 111 us the scores were 31, the values 26.
+// Two CTAs an SM with rings of eight pages and four with rings of three were no faster, nor was
+// a loop over page pairs; five stages cost 4 us with f32 outputs.
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
 constexpr int kStages = 4;  // even: pages are asked for in pairs (six do not fit three CTAs)
@@ -471,8 +474,8 @@ constexpr int kWideRowsBf16 = 64, kWideRowsF16 = 96;
 // (queries x n_head).  One sequence of 4000, 64/8 heads: of 128, 2048 rows take 98 us there and
 // 58 here, 4096 98 and 103; of 64, 4096 take 85 and 66, 8192 85 and 121.
 constexpr int64_t kWideTotal128 = 4096, kWideTotal64 = 6144;
-// What a unit costs beside its pages (queries, joins), in pages: 8 took 106 us for the first
-// of the cases above and 74 for the second, 16 takes 104 and 72, 24 the same.
+// What a unit costs beside its pages (queries, joins), in pages.  In an earlier version 8 took
+// 106 us for the first of the cases above and 74 for the second, 16 104 and 72, 24 the same.
 constexpr int kUnitCost = 16;
 // Units of up to so many pages are not split: the join costs 6 us (one sequence of 160 tokens:
 // 7 us whole, 13 split); 32 pages took 33 us for 8 sequences of 2000 and 4 queries, 16 31.
