@@ -279,8 +279,9 @@ rtd_status rtd_kv4_read(rtd_ctx* ctx, const int32_t* slots, int64_t n, int32_t n
  * 0 .. ctx_len[s] - n + i; a row that sees none is written as zeros, a row of no sequence
  * is left alone.  max_q and max_ctx bound the queries and the length of any sequence.
  * Accuracy: an f32 or f16 output is that of exact codes with queries and weights in 22 bits
- * or more and 32-bit sums, about 5e-7 of the result before its own rounding; a bf16 output
- * takes queries and weights in 11 bits.  With 16-bit outputs prompt chunks (sequences with
+ * or more and 32-bit sums, about 5e-7 of the result before its own rounding (1e-5 where the
+ * values are below 1e-6, the end of the headers' f16); a bf16 output takes queries and weights
+ * in 11 bits.  With 16-bit outputs prompt chunks (sequences with
  * 64 or more rows of queries x heads of the group, 96 with f16 outputs, at head_dim 64 or 128,
  * if they come to 6144 or 4096 rows of queries x n_head in all) take queries, weights, keys
  * and values rounded to f16: f16 outputs are then about 6e-4 of 64 bits, where those above are

@@ -567,13 +567,13 @@ struct Attn {
   static constexpr int kPart = kRows * (D + 2);
   static constexpr int kJoinBytes = kAttnWarps * kState * 4;
   static constexpr int kCols = EXACT ? 2 : 4;  // sums of a fragment: of both row halves, or as the MMA has them
-  static constexpr int kSmem = kAttnWarps * kStages * PB + kJoinBytes + NG * 1024 + 4 * kAttnWarps;
+  static constexpr int kSmem = kAttnWarps * kStages * PB + kJoinBytes + NG * 1024 + 4 * NG * kAttnWarps;
   const Kv4AttnArgs& a;
   uint8_t* ring;      // this warp's pages
   uint32_t ring32;
   uint64_t* bars;     // and their barriers
   float* join;        // the warps' states
-  uint32_t qfrag;     // this lane's query fragments, [group][k step][lane][16 bytes]; behind them the warps' lifts
+  uint32_t qfrag;     // this lane's query fragments, [group][k step][lane][16 bytes]; behind them the warps' scales
   int G, lane, warp;
   int wide_rows = INT32_MAX;    // a.wide_rows where the chunks are many enough
   unsigned get = 0, phase = 0;  // the ring's next page to use, and its parity
@@ -768,12 +768,13 @@ struct Attn {
 
   // O += (p d) C and the header sums z of a page, p = ph + pl of pairs of tokens (i, i + 4) and
   // (i + 8, i + 12).
-  __device__ void values(uint32_t page, bool large, int r, int qi, const uint32_t (&ph)[2], const uint32_t (&pl)[2],
+  template <bool SECOND>
+  __device__ void values(uint32_t page, int r, int qi, const uint32_t (&ph)[2], const uint32_t (&pl)[2],
                          float (&o)[NG][4][kCols], float (&z)[4]) const {
     // ---- sums of p times what a group's codes add to: its minimum, or, about code 8, the
     // middle m + 8 d.  The middles lie around zero, where the sums of the minima and of the
     // steps would each grow and then cancel; column g takes the middle as f16, column 4 + g
-    // the rest (two-sum).  Where m + 8 d may pass f16's range (`large`), a 16th.
+    // the rest (two-sum).  On a second attempt a 16th where m + 8 d would pass f16's range.
     const uint32_t vh = page + 18 * D;
     {
       const int g = min(r & 3, NG - 1);
@@ -784,7 +785,11 @@ struct Attn {
         const uint32_t w0 = lds(at + 32 * NG * u), w1 = lds(at + 32 * NG * u + 16 * NG);
         b[u] = prmt(w0, w1, 0x7632u);
         if constexpr (EXACT) {
-          const __half2 s8 = __float2half2_rn(large ? 0.5f : 8.0f), s1 = __float2half2_rn(large ? 0.0625f : 1.0f);
+          __half2 s8 = __float2half2_rn(8.0f), s1 = __float2half2_rn(1.0f);
+          if constexpr (SECOND) {
+            s1 = __high2half2(as_h2(lds(scales_at() + 4 * g)));
+            s8 = __hmul2_rn(s8, s1);
+          }
           const __half2 x = __hmul2_rn(as_h2(prmt(w0, w1, 0x5410u)), s8), y = __hmul2_rn(as_h2(b[u]), s1);
           const __half2 sum = __hadd2_rn(x, y), v = __hsub2_rn(sum, x);
           const __half2 rest = __hadd2_rn(__hsub2_rn(x, __hsub2_rn(sum, v)), __hsub2_rn(y, v));
@@ -794,6 +799,11 @@ struct Attn {
       if constexpr (EXACT) {
         float t[4];
         mma0(t, ph[0], pl[0], ph[1], pl[1], b[0], b[1]);
+        if constexpr (SECOND) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (lds(scales_at() + 4 * min(2 * (qi & 1) + (c & 1), NG - 1)) >> 16 != 0x3c00u) t[c] *= 16.0f;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) z[c] += t[c];
       } else {
@@ -813,14 +823,19 @@ struct Attn {
         if constexpr (NG & 1) vw[c][NG / 2] = lds_half(vr + ((NG - 1) * 8 + r) * 2);
       }
     }
-    const __half2 lift = as_h2(EXACT ? lds(lift_at()) : 0u);
+    // one for all groups, or one each
+    uint32_t scales[NG] = {};
+    if constexpr (SECOND)
+      lds_row<NG>(scales_at(), scales);
+    else if constexpr (EXACT)
+      scales[0] = lds(scales_at());
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       uint32_t hi[2], lo[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         __half2 d = as_h2(prmt(vd[2 * u][g], vd[2 * u + 1][g], 0x5410u));
-        if constexpr (EXACT) d = __hmul2(d, lift);
+        if constexpr (SECOND || EXACT) d = __hmul2(d, __low2half2(as_h2(scales[SECOND ? g : 0])));
         const __half2 p = as_h2(ph[u]), h = __hmul2(p, d);
         hi[u] = as_u32(h);
         lo[u] = EXACT ? as_u32(__hfma2(as_h2(pl[u]), d, __hfma2(p, d, __hneg2(h)))) : 0u;
@@ -834,10 +849,20 @@ struct Attn {
     }
   }
 
-  // Small steps are lifted by a power of two, at most 2^15: the rest of p d lies on f16's grid of
-  // 2^-24, which with p d of 2^-7 was 4e-6 of it.  The largest step of a warp's first page (the
-  // keys that any row sees) goes to 2^-4 .. 2^-3, and later ones may be 256 times as large.
-  __device__ int lift_of(uint32_t vh, int keys) const {
+  // Steps are lifted by a power of two, at most 2^15: the rest of p d lies on f16's grid of 2^-24,
+  // which with p d of 2^-7 was 4e-6 of it.  The largest step of a warp's first page that holds any
+  // (of the keys that some row sees) goes to 2^-4 at least, and later ones may be 256 times as
+  // large; on the second attempt, with p at most 1, every group of every page goes to 2^14 where
+  // 2^15 suffice.
+  // A warp's words, f16 pairs: 2^lift of a group's steps, and what its middles are multiplied by.
+  // In shared memory, since the loop over the pages has no register left.
+  __device__ uint32_t scales_at() const { return qfrag - 16 * lane + NG * 1024 + 4 * NG * warp; }
+  __device__ int lift_now(int g) const { return (int)(lds(scales_at() + 4 * g) >> 10 & 31u) - 15; }
+  __device__ void set_scales(int g, uint32_t factors) const {
+    if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(scales_at() + 4 * g), "r"(factors) : "memory");
+  }
+  // False: the page holds no step above zero.
+  __device__ bool first_scales(uint32_t vh, int keys) const {
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < (16 * NG + 31) / 32; ++i) {
@@ -846,21 +871,40 @@ struct Attn {
       if (d < 0x7c00u) most = max(most, d);
     }
     most = __reduce_max_sync(0xffffffffu, most);
-    return most ? max(0, min(15, -4 - ilogbf(f16_bits_to_f32(most)))) : 0;
-  }
-  // Kept in shared memory, an f16 pair of 2^lift: the loop over the pages has no register left.
-  __device__ uint32_t lift_at() const { return qfrag - 16 * lane + NG * 1024 + 4 * warp; }
-  __device__ void set_lift(int by) const {
+    if (!most) return false;
+    const uint32_t by = (uint32_t)max(0, min(15, -4 - ilogbf(f16_bits_to_f32(most))));
+#pragma unroll
+    for (int g = 0; g < NG; ++g) set_scales(g, (by + 15) << 10 | 0x3c000000u);
     __syncwarp();
-    if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(lift_at()), "r"(0x3c003c00u + by * 0x04000400u) : "memory");
+    return true;
+  }
+  // The second attempt's, and the sums so far in their terms.
+  __device__ void page_scales(uint32_t vh, int keys, float (&o)[NG][4][kCols]) const {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t h = lane < min(kTok, keys) ? lds(vh + 4 * (lane * NG + g)) & 0x7fff7fffu : 0u;
+      const bool number = (h & 0x7fffu) < 0x7c00u && h >> 16 < 0x7c00u;
+      const float d = f16_bits_to_f32(__reduce_max_sync(0xffffffffu, number ? h & 0xffffu : 0u));
+      const float m = f16_bits_to_f32(__reduce_max_sync(0xffffffffu, number ? h >> 16 : 0u));
+      const int now = lift_now(g), to = d > 0.0f ? min(now, max(0, 14 - ilogbf(d))) : now;
+      if (to < now) {
+        const float f = pow2(to - now);
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) o[g][p][c] *= f;
+      }
+      __syncwarp();
+      set_scales(g, (uint32_t)(to + 15) << 10 | (fmaf(8.0f, d, m) > 32768.0f ? 0x2c000000u : 0x3c000000u));
+    }
     __syncwarp();
   }
-  __device__ int lift_now() const { return (int)(lds(lift_at()) >> 26) - 15; }
 
   // A page with keys that some row does not see: such keys weigh nothing, whatever they hold,
   // so V headers that are not finite are zeroed, since 0 * NaN would reach every row of the
-  // MMA; a row that does see such a header gets its group's NaN here.
-  __device__ void sanitise(uint32_t vh, int key, int limit, float (&o)[NG][4][kCols]) const {
+  // MMA; a row that does see such a header gets its group's NaN here.  Headers of keys that no row
+  // of the tile sees are zeroed too: the steps are scaled by the others'.
+  __device__ void sanitise(uint32_t vh, int key, int most, int limit, float (&o)[NG][4][kCols]) const {
     uint64_t nan_at = 0;
 #pragma unroll
     for (int i = 0; i < (16 * NG + 31) / 32; ++i) {
@@ -869,7 +913,7 @@ struct Attn {
       if (at < 16 * NG) {
         const uint32_t h = lds(vh + 4 * at);
         no = (h & 0x7c00u) == 0x7c00u || (h & 0x7c000000u) == 0x7c000000u;
-        if (no) asm volatile("st.shared.u32 [%0], %1;" ::"r"(vh + 4 * at), "r"(0u) : "memory");
+        if (no || key + at / NG >= most) asm volatile("st.shared.u32 [%0], %1;" ::"r"(vh + 4 * at), "r"(0u) : "memory");
       }
       nan_at |= (uint64_t)__ballot_sync(0xffffffffu, no) << (32 * i);
     }
@@ -887,10 +931,96 @@ struct Attn {
     __syncwarp();
   }
 
+  // One attempt: p = 2^(x - max + headroom) right after a maximum is set, which stays until a score
+  // would pass 2^growth.
+  template <bool SECOND>
+  __device__ void walk(Seg& sg, const uint32_t (&qm)[3], float rowmul, int least, int most, int limit, float& M, float& l,
+                       float (&o)[NG][4][kCols], float (&z)[4]) {
+    const int mine = sg.mine, first = sg.first;
+    const int r = lane >> 2, qi = lane & 3;
+    const int kt = ((r & 1) << 2) | (r >> 1);  // token of S column r: columns 2 i, 2 i + 1 are tokens i, i + 4
+    constexpr float headroom = SECOND ? 0.0f : 8.0f, growth = SECOND ? 0.0f : 12.0f;
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < NG; ++g) set_scales(g, SECOND || EXACT ? 0x3c007800u : 0x3c003c00u);  // 2^15 or 1, and 1
+    __syncwarp();
+    bool scaled = false;
+    M = -1e30f;
+    l = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) z[c] = 0.0f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[g][p][c] = 0.0f;
+    for (int j = 0; j < mine; ++j) {
+      mbar_wait_bounded(bars + get, phase, a.status);
+      const uint32_t page = ring32 + get * PB;
+      if (++get == kStages) {
+        get = 0;
+        phase ^= 1;
+      }
+      const int key = (first + j * kAttnWarps) * kTok;
+      // ---- scores
+      float x[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) *reinterpret_cast<float2*>(x[u]) = unf2(scores(page, u, kt, qi, qm));
+      if (key + kTok > least) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            if (key + 8 * u + 4 * c + qi >= limit) x[u][c] = -INFINITY;
+        sanitise(page + 18 * D, key, most, limit, o);
+      }
+      // ---- running softmax
+      float mx = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])) * rowmul;
+      if (__any_sync(0xffffffffu, mx > M + growth)) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (mx > M + growth) {
+          const float to = mx - headroom, f = ex2(M - to);
+          M = to;
+          l *= f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) z[c] *= f;
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) o[g][p][c] *= f;
+        }
+      }
+      uint32_t ph[2], pl[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float p0 = ex2(fmaf(x[u][0], rowmul, -M)), p1 = ex2(fmaf(x[u][1], rowmul, -M));
+        l += p0 + p1;
+        const __half2 h = __floats2half2_rn(p0, p1);
+        ph[u] = as_u32(h);
+        pl[u] = 0;
+        if constexpr (EXACT) {
+          const float2 f = __half22float2(h);
+          pl[u] = as_u32(__floats2half2_rn(p0 - f.x, p1 - f.y));
+        }
+      }
+      if constexpr (SECOND)
+        page_scales(page + 18 * D, most - key, o);
+      else if (EXACT && !scaled)
+        scaled = first_scales(page + 18 * D, most - key);
+      values<SECOND>(page, r, qi, ph, pl, o, z);
+      __syncwarp();
+      if (j & 1) issue(sg, j + kStages - 1);  // the two pages just used
+    }
+  }
+
   // This warp's pages of the stretch: per row the running maximum M and sum l, and in
   // fragments the products o and the header sums z.
   __device__ void pages(Seg& sg, float& M, float& l, float (&o)[NG][4][kCols], float (&z)[4]) {
-    const int qs = sg.qs, kvh = sg.kvh, mine = sg.mine, first = sg.first;
+    const int qs = sg.qs, kvh = sg.kvh, mine = sg.mine;
     const int row0 = sg.tile * kRows, rows = sg.nq * G;
     const int least = seen(sg, row0), most = seen(sg, min(row0 + kRows, rows) - 1);
     // ---- queries: lane (row r, quad lane i) holds dims 8 i .. 8 i + 7 of every group
@@ -973,104 +1103,24 @@ struct Attn {
       }
     }
 
-    const int kt = ((r & 1) << 2) | (r >> 1);  // token of S column r: columns 2 i, 2 i + 1 are tokens i, i + 4
-    // p = 2^(x - max + headroom) right after a maximum is set, which stays until a score
-    // would pass 2^growth; if p d left f16's range after all, the pages are read once more
-    // without the lift and, if that was not it (a step above 16), with p at most 1
-    if (EXACT) set_lift(0);
-    for (int attempt = 0;; ++attempt) {
-      const float headroom = attempt == 2 ? 0.0f : 8.0f, growth = attempt == 2 ? 0.0f : 12.0f;
-      M = -1e30f;
-      l = 0.0f;
+    walk<false>(sg, qm, rowmul, least, most, limit, M, l, o, z);
+    if (mine == 0) return;
+    // if p d or a middle left f16's range after all (a step above 16, or 256 times the first page's),
+    // the pages are read once more with p at most 1 and the scales found for every page
+    float probe = 0.0f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) z[c] = 0.0f;
+    for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
+      for (int p = 0; p < 4; ++p)
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
+        for (int c = 0; c < kCols; ++c) probe = fmaf(o[g][p][c], 0.0f, probe);
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) o[g][p][c] = 0.0f;
-      for (int j = 0; j < mine; ++j) {
-        mbar_wait_bounded(bars + get, phase, a.status);
-        const uint32_t page = ring32 + get * PB;
-        if (++get == kStages) {
-          get = 0;
-          phase ^= 1;
-        }
-        const int key = (first + j * kAttnWarps) * kTok;
-        // ---- scores
-        float x[2][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) *reinterpret_cast<float2*>(x[u]) = unf2(scores(page, u, kt, qi, qm));
-        if (key + kTok > least) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-              if (key + 8 * u + 4 * c + qi >= limit) x[u][c] = -INFINITY;
-          sanitise(page + 18 * D, key, limit, o);
-        }
-        // ---- running softmax
-        float mx = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])) * rowmul;
-        if (__any_sync(0xffffffffu, mx > M + growth)) {
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          if (mx > M + growth) {
-            const float to = mx - headroom, f = ex2(M - to);
-            M = to;
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) z[c] *= f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-              for (int p = 0; p < 4; ++p)
-#pragma unroll
-                for (int c = 0; c < kCols; ++c) o[g][p][c] *= f;
-          }
-        }
-        uint32_t ph[2], pl[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float p0 = ex2(fmaf(x[u][0], rowmul, -M)), p1 = ex2(fmaf(x[u][1], rowmul, -M));
-          l += p0 + p1;
-          const __half2 h = __floats2half2_rn(p0, p1);
-          ph[u] = as_u32(h);
-          pl[u] = 0;
-          if constexpr (EXACT) {
-            const float2 f = __half22float2(h);
-            pl[u] = as_u32(__floats2half2_rn(p0 - f.x, p1 - f.y));
-          }
-        }
-        if constexpr (EXACT)
-          if (j == 0 && attempt == 0) set_lift(lift_of(page + 18 * D, most - key));
-        values(page, attempt == 2, r, qi, ph, pl, o, z);
-        __syncwarp();
-        if (j & 1) issue(sg, j + kStages - 1);  // the two pages just used
-      }
-      if (attempt == 2) {
-        if constexpr (EXACT)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) z[c] *= 16.0f;
-        break;
-      }
-      if (mine == 0) break;
-      float probe = 0.0f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) probe = fmaf(o[g][p][c], 0.0f, probe);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) probe = fmaf(z[c], 0.0f, probe);
-      if (!__any_sync(0xffffffffu, probe != 0.0f)) break;  // NaN where anything was not finite
-      if (!EXACT || lift_now() == 0) attempt = 1;
-      if (EXACT) set_lift(0);
-      // from the start once more: the ring is empty, and an odd number of pages may have used it
-      sg.ids = load_ids(sg, 0);
-      for (int j = 0; j < kStages; j += 2) issue(sg, j);
-    }
+    for (int c = 0; c < 4; ++c) probe = fmaf(z[c], 0.0f, probe);
+    if (!__any_sync(0xffffffffu, probe != 0.0f)) return;  // NaN where anything was not finite
+    // from the start: the ring is empty, and an odd number of pages may have used it
+    sg.ids = load_ids(sg, 0);
+    for (int j = 0; j < kStages; j += 2) issue(sg, j);
+    walk<true>(sg, qm, rowmul, least, most, limit, M, l, o, z);
   }
 
   // Joins the warps' states into the output or, where the unit goes on in other CTAs, into a
@@ -1087,7 +1137,6 @@ struct Attn {
     }
     {
       float* out = join + warp * kState + r * kPitch + 8 * qi;
-      const float down = EXACT ? pow2(-lift_now()) : 1.0f;
       const float z0 = z[0] + z[2], z1 = z[1] + z[3];  // quad lanes 0, 1: middles or minima; 2, 3: their rests
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -1095,10 +1144,11 @@ struct Attn {
         const float zm = __shfl_sync(0xffffffffu, (g & 1) ? z1 : z0, from);
         const float zd = __shfl_sync(0xffffffffu, (g & 1) ? z1 : z0, from + 2);
         const float zz = EXACT ? zm + zd : zm;
+        const float down = pow2((EXACT ? 0 : 24) - lift_now(g));
         float v[8];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          const float f = (EXACT ? down : 16777216.0f) * ((p & 1) ? 0.0625f : 1.0f);  // the odd nibbles' 16
+          const float f = down * ((p & 1) ? 0.0625f : 1.0f);  // the odd nibbles' 16
           v[p] = fmaf(o[g][p][0] + (EXACT ? 0.0f : o[g][p][kCols - 2]), f, zz);
           v[4 + p] = fmaf(o[g][p][1] + (EXACT ? 0.0f : o[g][p][kCols - 1]), f, zz);
         }

@@ -104,3 +104,63 @@ def test_prompt_chunks(D, lens, new, out_dtype):
     for s, want in enumerate(wanted(c, q.astype(np.float64), new)):
         assert rel(got[at:at + new[s]] - want, want) <= limit, (s, rel(got[at:at + new[s]] - want, want))
         at += new[s]
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,n_kv,D", HEADS)
+@pytest.mark.parametrize("what,v_std", [(np.nan, 1e-4), (np.nan, 1.0), (1e5, 1e-2), ("grown", 1e-3), ("grown", 1.0)])
+def test_what_is_read_twice_loses_no_accuracy(H, n_kv, D, what, v_std, out_dtype):
+    # a NaN, a value beyond f16, or values 1e5 times those of a warp's first page
+    c = Case([700], n_kv, D, seed=3, v_std=v_std)
+    v = c.V[0].astype(np.float32)
+    if what == "grown":
+        v[:80] *= 1e-5
+    else:
+        v[400, 0, D - 1] = what
+    c.write(c.K[0].astype(np.float32), v, c.slots[0])
+    q = np.random.default_rng(1).normal(0, 1, (2, H, D)).astype(np.float32)
+    got = run_attention(c, dev(q), [2], out_dtype=out_dtype).double().cpu().numpy().reshape(2, H, D // 32, 32)
+    want = wanted(c, q.astype(np.float64), [2])[0].reshape(got.shape)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    limit = {torch.float32: 1e-6, torch.float16: 1e-6, torch.bfloat16: 2.6e-3}[out_dtype]
+    for g in range(D // 32):
+        for h in range(n_kv):
+            at = np.s_[:, h * (H // n_kv):(h + 1) * (H // n_kv), g]
+            if np.isnan(want[at]).any():
+                continue
+            err = got[at] - want[at]
+            if out_dtype == torch.float16:
+                err = np.maximum(0, np.abs(err) - np.abs(want[at]) * 2.0 ** -11 - 2.0 ** -25)
+            assert rel(err, want[at]) <= limit, (g, h, rel(err, want[at]))
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,n_kv,D", HEADS)
+@pytest.mark.parametrize("small,large,nan", [(1e-4, 1e3, None), (1e-3, 1e5, None), (1e-4, 1.0, 37), (1.0, 1e5, 30)])
+def test_large_values_of_keys_not_seen_yet(H, n_kv, D, small, large, nan, out_dtype):
+    # row by row: those before token 21 see small values alone, the others of its page are large
+    c = Case([40], n_kv, D, seed=5, v_std=1.0)
+    v = c.V[0].astype(np.float32)
+    v[:21] *= small
+    v[21:] *= large / 4
+    v[21:] = np.clip(v[21:], -60000, None)
+    if nan is not None:
+        v[nan, 0, 3] = np.nan
+    c.write(c.K[0].astype(np.float32), v, c.slots[0])
+    q = np.random.default_rng(2).normal(0, 1, (40, H, D)).astype(np.float32)
+    got = run_attention(c, dev(q), [40], out_dtype=out_dtype).double().cpu().numpy()
+    want = np.zeros(got.shape)
+    for i in range(40):
+        for h in range(H):
+            x = q[i, h].astype(np.float64) @ c.K[0][:i + 1, h * n_kv // H].T / math.sqrt(D)
+            w = np.exp(x - x.max())
+            want[i, h] = (w / w.sum()) @ c.V[0][:i + 1, h * n_kv // H]
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    # Eight rows (token * G + head) are read together.  Where 8 divides G they see the same keys, and
+    # each is as near as alone; elsewhere, as with G = 20, rows 416 .. 423 belong to tokens 20 and 21,
+    # and what f16 pairs hold beside values 1e8 times as large is all that remains of the first.
+    if H // n_kv % 8 == 0:
+        limit = 2e-6 if out_dtype == torch.float32 else 8e-3
+        ok = ~np.isnan(want).any(axis=(1, 2))
+        err = np.linalg.norm((got - want)[ok], axis=(1, 2)) / np.linalg.norm(want[ok], axis=(1, 2))
+        assert err.max() <= limit, (err.argmax(), err.max())
